@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256, 2) void k_chain(const float4 *chunks, float *o
                 }
                 if constexpr (c == 0 && TAPE != 0 && TAPE < 8) {
                     // TAPE bit 0: 16 float4 stores of the previous layer's output; bit 1: packed sign-bit words (v_cmp + or per
-                    // register, one 8-byte store); bit 2: sign bits as v_cmp lane masks stored with scalar stores
+                    // register, one 8-byte store)
                     if (l > 0) {
                         float *r = tape + ((long)(l & 7) * tape_rows + row) * 256 + 4 * part;
                         if constexpr (TAPE == 7) {          // non-temporal stores: keep the tape out of the L2 the weights live in
@@ -112,20 +112,6 @@ __global__ __launch_bounds__(256, 2) void k_chain(const float4 *chunks, float *o
 #pragma unroll
                             for (int i = 0; i < 32; ++i) { m0 |= h[i] > 0.f ? (1u << i) : 0u; m1 |= h[32 + i] > 0.f ? (1u << i) : 0u; }
                             *reinterpret_cast<uint2 *>(tape + (8 * tape_rows) * 256 + ((long)(l & 7) * tape_rows + row) * 8 + part * 2) = make_uint2(m0, m1);
-                        }
-                        if constexpr ((TAPE & 4) && TAPE != 7) {
-                            const size_t mpv = (size_t)(reinterpret_cast<unsigned long long *>(tape + (8 * tape_rows) * 256) +
-                                                        ((long)(l & 7) * (tape_rows / 16) + ((long)blockIdx.x * 4 + wave)) * 64);
-                            const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)mpv), hi = __builtin_amdgcn_readfirstlane((unsigned)(mpv >> 32));
-                            const unsigned long long mp = ((unsigned long long)hi << 32) | lo;
-#pragma unroll
-                            for (int i = 0; i < H / 2; ++i) {
-                                const unsigned long long b0 = __ballot(h[2 * i] > 0.f), b1 = __ballot(h[2 * i + 1] > 0.f);
-                                typedef unsigned uint4v __attribute__((ext_vector_type(4)));
-                                uint4v v = {(unsigned)b0, (unsigned)(b0 >> 32), (unsigned)b1, (unsigned)(b1 >> 32)};
-                                const unsigned off = (unsigned)(i * 16);
-                                asm volatile("s_store_dwordx4 %0, %1, %2" ::"s"(v), "s"(mp), "s"(off) : "memory");
-                            }
                         }
                     }
                 }
@@ -208,7 +194,6 @@ __global__ __launch_bounds__(256, 2) void k_chain(const float4 *chunks, float *o
         if constexpr (MODE == 3) __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (MODE != 0) wait_vm<0>();
-    if constexpr ((TAPE & 4) && TAPE != 7) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb" ::: "memory");
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < H; ++i) s += h[i];
@@ -268,8 +253,6 @@ int main(int argc, char **argv) {
         run<0, 1>(chunks, out, tape, rows, nl);
         run<0, 2>(chunks, out, tape, rows, nl);
         run<0, 3>(chunks, out, tape, rows, nl);
-        run<0, 4>(chunks, out, tape, rows, nl);
-        run<0, 5>(chunks, out, tape, rows, nl);
         run<0, 32>(chunks, out, tape, rows, nl);
         run<0, 33>(chunks, out, tape, rows, nl);
         run<1>(chunks, out, tape, rows, nl);
