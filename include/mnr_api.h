@@ -33,6 +33,13 @@ extern "C" {
 #define MNR_E_LAUNCH (-2)    /* HIP launch failure */
 #define MNR_E_UNSUPPORTED (-3)
 
+/* element types of the operators that take more than fp32 */
+#define MNR_F32 0
+#define MNR_F16 1
+#define MNR_BF16 2
+#define MNR_I32 3
+#define MNR_I64 4
+
 #define MNR_MAX_LAYERS 16
 
 int mnr_version(void);
@@ -191,6 +198,65 @@ int mnr_col_sum(float *out_dev, const float *G_dev, int64_t ldg, int64_t R, int 
 /* table_grad[idx[r / rows_per_ray]][0..width) += src[r][0..width)  (gradient of mnr_gather_rows) */
 int mnr_scatter_rows(float *table_grad_dev, int width, int count, const void *idx_dev, int64_t idx_stride, int idx_is_float,
                      int64_t rows_per_ray, const float *src_dev, int64_t ld_src, int64_t R, void *stream);
+/* ---- operators beside the layer-by-layer path: layer norm, embedding, gate, 8-bit product -----------------------------------
+ * Element types: MNR_F32, MNR_F16, MNR_BF16; sums and statistics are fp32 whatever the type, outputs are rounded once.  Rows may
+ * start at any element's address (pitches in elements, the last dimension contiguous).  Work on the caller's stream and memory
+ * only, no atomics in any sum: the same inputs give the same bits.  (csrc/layer_norm.hip, embedding.hip, gate.hip, int8_product.hip) */
+
+/* y = (x - mean) rstd w + b over the last dimension, rstd = 1 / sqrt(var + eps); w / b [cols] of type w_type, or NULL (1 / 0).
+ * mean / rstd [rows] are what the backward pass reads (NULL: not kept). */
+int mnr_layer_norm_forward(void *y_dev, int64_t ldy, float *mean_dev, float *rstd_dev, const void *x_dev, int64_t ldx, const void *w_dev,
+                           const void *b_dev, int64_t rows, int64_t cols, float eps, int type, int w_type, void *stream);
+/* dx (of x's type), dw and db (of w_type), each overwritten, each NULL if not wanted; the workspace is needed for dw / db only */
+size_t mnr_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int type);
+int mnr_layer_norm_backward(void *dx_dev, int64_t lddx, void *dw_dev, void *db_dev, const void *dy_dev, int64_t lddy, const void *x_dev,
+                            int64_t ldx, const void *w_dev, const float *mean_dev, const float *rstd_dev, int64_t rows, int64_t cols,
+                            int type, int w_type, void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* out[r] = scale table[idx[r]]; idx int32, int64 or fp32 (idx_type MNR_I32, MNR_I64, MNR_F32: the image index column of a ray).
+ * Indices outside the table are clamped, as in mnr_gather_rows. */
+int mnr_embedding_forward(void *out_dev, int64_t ldo, const void *table_dev, int64_t ldt, int64_t count, int64_t width, const void *idx_dev,
+                          int idx_type, float scale, int64_t rows, int type, void *stream);
+/* grad [count][width], dense and overwritten: grad[v] = scale sum of dy[r] over the rows r with idx[r] = v, in row order (the rows are
+ * sorted by index: mnr_scatter_rows adds them up with atomics instead).  The row of padding_idx (-1: none) stays zero.
+ * grad_type: type, or MNR_F32. */
+size_t mnr_embedding_backward_workspace_bytes(int64_t rows, int64_t count, int64_t width);
+int mnr_embedding_backward(void *grad_dev, int grad_type, const void *dy_dev, int64_t ldy, const void *idx_dev, int idx_type, int64_t rows,
+                           int64_t count, int64_t width, int64_t padding_idx, float scale, int type, void *workspace_dev,
+                           size_t workspace_bytes, void *stream);
+
+/* A learned gate over n_cells cells (mnr_route is the geometric one).  Open cells: mask set (NULL: all; ldm 0: one mask row for all
+ * rows) and logit > -inf.  s = softmax over the open cells (score 0) or sigmoid (score 1); v = s + bias (bias [n_cells] or NULL: the
+ * logits decide).  With n_groups > 1 only the k_groups groups stay open whose group_top (1 or 2) best s + bias sum highest.  Chosen:
+ * the k largest v, largest first, the lowest index of equals.  cells [rows][k] = their numbers, weights [rows][k] = scale s, divided
+ * by the chosen s' sum if renormalise.  Where fewer than k cells are open the rest of the slots is -1 with weight 0; a row with a NaN
+ * in an open logit (softmax: or +inf) has cells -1 and weights NaN.  k <= 32, n_cells <= 1024. */
+int mnr_gate_forward(float *weights_dev, int32_t *cells_dev, const void *logits_dev, int64_t ldl, const float *bias_dev,
+                     const uint8_t *mask_dev, int64_t ldm, int64_t rows, int n_cells, int k, int score, int n_groups, int k_groups,
+                     int group_top, int renormalise, float scale, int type, void *stream);
+/* dlogits [rows][n_cells] of the weights' gradient dweights [rows][k], the choice being fixed (cells as mnr_gate_forward wrote them;
+ * zero for a row without cells) */
+int mnr_gate_backward(void *dlogits_dev, int64_t ldd, const float *dweights_dev, int64_t lddw, const void *logits_dev, int64_t ldl,
+                      const int32_t *cells_dev, const uint8_t *mask_dev, int64_t ldm, int64_t rows, int n_cells, int k, int score,
+                      int renormalise, float scale, int type, void *stream);
+/* order [slots] = the slots sorted by cell, in slot order inside a cell, those without a cell (outside [0, n_cells)) last;
+ * cell c's are order[offsets[c]] ... order[offsets[c + 1] - 1], offsets [n_cells + 1] */
+size_t mnr_gate_dispatch_workspace_bytes(int64_t slots, int n_cells);
+int mnr_gate_dispatch(int32_t *order_dev, int32_t *offsets_dev, const int32_t *cells_dev, int64_t slots, int n_cells, void *workspace_dev,
+                      size_t workspace_bytes, void *stream);
+
+/* values [rows][pitch] = round(127 x / max|row|) to the nearest, ties to even, scale [rows] = max|row| / 127; a row of zeros has scale
+ * 0, a row with an inf or NaN scale NaN and values 0.  Columns cols .. pitch are zeroed; pitch is a multiple of 16. */
+int mnr_quantize_rows(int8_t *values_dev, int64_t pitch, float *scale_dev, const void *x_dev, int64_t ldx, int64_t rows, int64_t cols,
+                      int type, void *stream);
+/* y[m][n] = act( a_scale[m] b_scale[n] sum_k a[m][k] b[n][k] + bias[n] ), the sum exact in int32 (k <= 131071); act: 0 none, 1 ReLU.
+ * a / b start at a multiple of 16 bytes with pitches that are multiples of 16; where k is no multiple of 16, a's rows (not b's) are
+ * zero behind column k, and both can be read up to the next multiple of 16. */
+size_t mnr_int8_product_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int mnr_int8_product(void *y_dev, int64_t ldy, const int8_t *a_dev, int64_t lda, const float *a_scale_dev, const int8_t *b_dev, int64_t ldb,
+                     const float *b_scale_dev, const float *bias_dev, int64_t m, int64_t n, int64_t k, int act, int type,
+                     void *workspace_dev, size_t workspace_bytes, void *stream);
+
 /* ---- wide layers of the layer-by-layer path: tiled GEMM with fused epilogues (csrc/tgemm.hip) and batched weight
  * gradients (csrc/wgrad.hip); what nerf.py:115-160 + autograd get from cuBLAS, for layer widths that are multiples of 256.
  *   C[m][n] = gate( relu( sum_p sum_k a[p][m][k] B_p(n,k) + bias[n] + r1_row[m] r1_col[n] ) )

@@ -212,6 +212,9 @@ EXPORTS = [
     'mnr_step_query', 'mnr_step_create', 'mnr_step_destroy', 'mnr_step_repack', 'mnr_train_step', 'mnr_step_profile', 'mnr_step_kernel_times',
     'mnr_packed_model_h2_bytes', 'mnr_pack_model_h2', 'mnr_mlp_forward_multi_h2', 'mnr_render_workspace_bytes', 'mnr_render_fwd', 'mnr_packed_bwd_h2_bytes', 'mnr_pack_model_bwd_h2',
     'mnr_mlp_backward_weights_multi_h2', 'mnr_mlp_forward_cells_h2', 'mnr_side_create', 'mnr_side_destroy', 'mnr_mlp_forward_cells_multi',
+    'mnr_layer_norm_forward', 'mnr_layer_norm_backward_workspace_bytes', 'mnr_layer_norm_backward', 'mnr_embedding_forward',
+    'mnr_embedding_backward_workspace_bytes', 'mnr_embedding_backward', 'mnr_gate_forward', 'mnr_gate_backward',
+    'mnr_gate_dispatch_workspace_bytes', 'mnr_gate_dispatch', 'mnr_quantize_rows', 'mnr_int8_product_workspace_bytes', 'mnr_int8_product',
     'mnr_calibrate', 'mnr_calibrate_scratch_bytes', 'mnr_calibrate_hog', 'mnr_render_route_workspace_bytes',
 ]
 
@@ -349,6 +352,24 @@ def lib() -> C.CDLL:
         _lib.mnr_step_kernel_times.argtypes = [C.c_void_p, C.c_int, c_float_p]
         _lib.mnr_train_step.argtypes = [C.c_void_p, C.POINTER(StepBatch), C.POINTER(StepRandoms), C.c_double, C.c_int64, C.c_uint64, C.c_int,
                                         C.c_void_p]
+        p, i64, i32, f32, size = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
+        _lib.mnr_layer_norm_forward.argtypes = [p, i64, p, p, p, i64, p, p, i64, i64, f32, i32, i32, p]
+        _lib.mnr_layer_norm_backward_workspace_bytes.restype = size
+        _lib.mnr_layer_norm_backward_workspace_bytes.argtypes = [i64, i64, i32]
+        _lib.mnr_layer_norm_backward.argtypes = [p, i64, p, p, p, i64, p, i64, p, p, p, i64, i64, i32, i32, p, size, p]
+        _lib.mnr_embedding_forward.argtypes = [p, i64, p, i64, i64, i64, p, i32, f32, i64, i32, p]
+        _lib.mnr_embedding_backward_workspace_bytes.restype = size
+        _lib.mnr_embedding_backward_workspace_bytes.argtypes = [i64, i64, i64]
+        _lib.mnr_embedding_backward.argtypes = [p, i32, p, i64, p, i32, i64, i64, i64, i64, f32, i32, p, size, p]
+        _lib.mnr_gate_forward.argtypes = [p, p, p, i64, p, p, i64, i64, i32, i32, i32, i32, i32, i32, i32, f32, i32, p]
+        _lib.mnr_gate_backward.argtypes = [p, i64, p, i64, p, i64, p, p, i64, i64, i32, i32, i32, i32, f32, i32, p]
+        _lib.mnr_gate_dispatch_workspace_bytes.restype = size
+        _lib.mnr_gate_dispatch_workspace_bytes.argtypes = [i64, i32]
+        _lib.mnr_gate_dispatch.argtypes = [p, p, p, i64, i32, p, size, p]
+        _lib.mnr_quantize_rows.argtypes = [p, i64, p, p, i64, i64, i64, i32, p]
+        _lib.mnr_int8_product_workspace_bytes.restype = size
+        _lib.mnr_int8_product_workspace_bytes.argtypes = [i64, i64, i64]
+        _lib.mnr_int8_product.argtypes = [p, i64, p, i64, p, p, i64, p, p, i64, i64, i64, i32, i32, p, size, p]
         _lib.mnr_calibrate_scratch_bytes.restype = C.c_size_t
         _lib.mnr_calibrate.argtypes = [C.POINTER(Calibration), C.c_void_p, C.c_size_t, C.c_void_p]
         _lib.mnr_calibrate_hog.argtypes = [C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_void_p]
@@ -364,6 +385,59 @@ def require_device(t: torch.Tensor, name: str = 'tensor') -> None:
     if not t.is_cuda:
         raise NativeError('{} must live on the HIP device (got {}); the MI355X kernels have no CPU fallback'.format(
             name, t.device))
+
+
+ELEMENT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}         # MNR_F32, MNR_F16, MNR_BF16
+INDEX_TYPES = {torch.float32: 0, torch.int32: 3, torch.int64: 4}                # MNR_F32, MNR_I32, MNR_I64
+
+
+def element_type(t: torch.Tensor, name: str) -> int:
+    """MNR_F32 / F16 / BF16 of a device tensor; raises for tensors on the CPU and for other types."""
+    code = ELEMENT_TYPES.get(t.dtype)
+    if code is None:
+        raise NativeError('{} must be float32, float16 or bfloat16 (got {})'.format(name, t.dtype))
+    if not t.is_cuda:
+        require_device(t, name)
+    return code
+
+
+def on_device_of(t: torch.Tensor, other: Optional[torch.Tensor], name: str) -> None:
+    if other is not None and other.device != t.device:
+        raise NativeError('{} is on {}, the input on {}'.format(name, other.device, t.device))
+
+
+def matrix(t: torch.Tensor):
+    """[..., C] -> (tensor with contiguous last dimension whose rows are one pitch apart, rows, C, pitch in elements).  Views that no
+    single pitch describes are copied."""
+    C_ = t.shape[-1]
+    if t.dim() == 2:
+        if t.stride(1) == 1 or C_ == 1:
+            if t.shape[0] <= 1:
+                return t, t.shape[0], C_, C_
+            if t.stride(0) >= C_:
+                return t, t.shape[0], C_, t.stride(0)
+    elif t.is_contiguous():
+        return t, t.numel() // C_ if C_ else 0, C_, C_
+    t = t.contiguous()
+    return t, t.numel() // C_ if C_ else 0, C_, C_
+
+
+def launch(t: torch.Tensor, fn, *args) -> None:
+    """Call a C entry point on the current stream of the device that ``t`` lives on."""
+    if t.device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(t.device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        check(rc)
+
+
+def refuse_captured_backward(what: str) -> None:
+    """Autograd's own bookkeeping may tie a captured backward pass to the stream of an earlier eager graph over the same parameters,
+    which ends the capture (and can end the process); the explicit ``*_backward`` calls have no such tie."""
+    if torch.cuda.is_current_stream_capturing():
+        raise NativeError('the backward pass of {0} through autograd is not captured into a HIP graph: record {0}_backward'.format(what))
 
 
 def stream_ptr() -> int:

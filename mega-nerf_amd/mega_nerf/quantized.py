@@ -1,0 +1,111 @@
+"""Matrix product in 8-bit integers with a scale for every row of the input and every output channel (csrc/int8_product.hip): the dense
+layers of a wide model served at a quarter of the bytes and on the 8-bit matrix pipe, beside the fp32 products of csrc/tgemm.hip and
+csrc/layerwise.hip.  Inference only: quantisation has no gradient here."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from mega_nerf import _native as N
+
+_PITCH = 128                 # rows of quantised values start at multiples of this many bytes
+
+
+class QuantizedRows(NamedTuple):
+    """``values`` int8 [rows, cols] and ``scale`` float32 [rows]: row r stands for scale[r] * values[r]."""
+    values: torch.Tensor
+    scale: torch.Tensor
+
+    def dequantize(self) -> torch.Tensor:
+        return self.values.float() * self.scale[:, None]
+
+
+def quantize_rows(x: torch.Tensor) -> QuantizedRows:
+    """``x`` [rows, cols] (float32, float16, bfloat16) with the scale max|row| / 127 for each row; values are rounded to the nearest,
+    ties to even.  A row of zeros gets scale 0; a row that holds an inf or NaN gets scale NaN.  A weight [out, in] is quantised the
+    same way, once: its rows are the output channels.  The values' rows start 128 bytes apart or a multiple of it, zeros in between
+    (what the product reads fastest)."""
+    code = N.element_type(x, 'x')
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise N.NativeError('quantize_rows expects [rows, cols] with a column at least (got {})'.format(tuple(x.shape)))
+    x, rows, cols, ldx = N.matrix(x.detach())
+    pitch = (cols + _PITCH - 1) // _PITCH * _PITCH
+    values = torch.empty(rows, pitch, dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    N.launch(x, N.lib().mnr_quantize_rows, values.data_ptr(), pitch, scale.data_ptr(), x.data_ptr(), ldx, rows, cols, code)
+    return QuantizedRows(values[:, :cols] if pitch > cols else values, scale)
+
+
+def _operand(q: QuantizedRows, name: str, zero_tail: bool):
+    """(tensor, rows, cols, pitch) of values that the kernel can read as they lie, else of a copy: 16-byte aligned rows, readable up to
+    the next multiple of 16 columns, and for the left operand zeros there (its tail cannot be known, so it is copied)."""
+    v, s = q
+    if v.dtype != torch.int8 or v.dim() != 2 or v.shape[1] == 0:
+        raise N.NativeError('{}.values must be int8 [rows, cols] with a column at least (got {} {})'.format(name, v.dtype, tuple(v.shape)))
+    if not v.is_cuda:
+        N.require_device(v, name + '.values')
+    if s.dtype != torch.float32 or s.shape != v.shape[:1]:
+        raise N.NativeError('{}.scale must be float32 [{}] (got {} {})'.format(name, v.shape[0], s.dtype, tuple(s.shape)))
+    N.on_device_of(v, s, name + '.scale')
+    rows, cols = v.shape
+    pitch, up = v.stride(0), (cols + 15) // 16 * 16
+    if rows <= 1:
+        pitch = max(pitch, up) // 16 * 16 if pitch % 16 else max(pitch, up)
+    ok = (v.stride(1) == 1 and pitch % 16 == 0 and pitch >= up and v.data_ptr() % 16 == 0 and not (zero_tail and up > cols) and
+          v.storage_offset() + max(rows - 1, 0) * pitch + up <= v.untyped_storage().nbytes())
+    if not ok:
+        pitch = (cols + _PITCH - 1) // _PITCH * _PITCH
+        held = torch.zeros(rows, pitch, dtype=torch.int8, device=v.device)
+        held[:, :cols] = v
+        v = held
+    return v, rows, cols, pitch
+
+
+def _product(a, m, k, lda, a_scale, b: QuantizedRows, bias, relu, out_dtype) -> torch.Tensor:
+    bv, n, kb, ldb = _operand(b, 'weight', False)
+    N.on_device_of(a, bv, 'weight')
+    if kb != k:
+        raise N.NativeError('the input has {} columns, the weight {}'.format(k, kb))
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (n,):
+            raise N.NativeError('bias must be float32 [{}] (got {} {})'.format(n, bias.dtype, tuple(bias.shape)))
+        N.on_device_of(a, bias, 'bias')
+        bias = bias.detach().contiguous()
+    code = N.ELEMENT_TYPES.get(out_dtype)
+    if code is None:
+        raise N.NativeError('the output is float32, float16 or bfloat16 (got {})'.format(out_dtype))
+    a_scale, b_scale = a_scale.contiguous(), b.scale.contiguous()
+    y = torch.empty(m, n, dtype=out_dtype, device=a.device)
+    lib = N.lib()
+    size = lib.mnr_int8_product_workspace_bytes(m, n, k)
+    ws = torch.empty(size, dtype=torch.uint8, device=a.device) if size else None
+    N.launch(a, lib.mnr_int8_product, y.data_ptr(), n, a.data_ptr(), lda, a_scale.data_ptr(), bv.data_ptr(), ldb, b_scale.data_ptr(),
+             N.ptr(bias), m, n, k, 1 if relu else 0, code, N.ptr(ws), size)
+    return y
+
+
+def int8_product(a: QuantizedRows, b: QuantizedRows, bias: Optional[torch.Tensor] = None, relu: bool = False,
+                 out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """[M, N] = a [M, K] times the transpose of b [N, K] (+ bias float32 [N], ReLU): the integer sums are exact (K <= 131071), scaled in
+    fp32 and rounded once to ``out_dtype``."""
+    av, m, k, lda = _operand(a, 'a', True)
+    return _product(av, m, k, lda, a.scale, b, bias, relu, out_dtype)
+
+
+def int8_linear(x: torch.Tensor, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, relu: bool = False,
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """A dense layer served in 8 bits: x [..., K] is quantised row by row, multiplied with ``weight`` = ``quantize_rows(w)`` of an
+    nn.Linear weight [N, K], scaled, ``bias`` added, ReLU if ``relu``; [..., N] of x's type, or ``out_dtype``."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError('int8_linear is inference-only (use torch.no_grad())')
+    N.element_type(x, 'x')
+    shape = x.shape
+    if x.dim() != 2:
+        if x.dim() == 0 or shape[-1] == 0:
+            raise N.NativeError('int8_linear expects [..., K] with a column at least (got {})'.format(tuple(shape)))
+        x = x.reshape(-1, shape[-1])
+    q = quantize_rows(x)
+    m, k = q.values.shape
+    y = _product(q.values, m, k, (k + _PITCH - 1) // _PITCH * _PITCH, q.scale, weight, bias, relu, x.dtype if out_dtype is None else out_dtype)
+    return y if len(shape) == 2 else y.view(*shape[:-1], y.shape[1])
