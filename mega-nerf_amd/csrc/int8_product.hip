@@ -86,70 +86,254 @@ struct ProductArgs {
     int relu;
 };
 
-template <class T> __device__ __forceinline__ void put_product(const ProductArgs &p, int64_t m, int64_t n, int acc, float sa, float sb, float bias) {
-    float y = (float)acc * sa * sb + bias;
-    if (p.relu) y = y < 0.f ? 0.f : y;
-    reinterpret_cast<T *>(p.y)[m * p.ldy + n] = (T)y;
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef __attribute__((address_space(1))) const void global_cvoid_t;
+
+// ---- the tiled product ------------------------------------------------------------------------------------------------------------
+// WR x WC waves, each with RB x CB blocks of 32 x 32 of the output.  K goes by in steps of 64 bytes through a ring of four LDS stages:
+// while step k multiplies, both operands' 64 bytes of every row of step k + 3 are fetched straight into LDS (16 bytes a lane, no
+// registers), a few fetches at a time between the matrix instructions: all at once they fill the fetch queue, and the waves wait to
+// issue instead of multiplying.  A stage is read as ds_read_b128 fragments of v_mfma_i32_32x32x32_i8, one set ahead of its use.  The
+// stages are separate LDS objects, so that the compiler's waits tell the fetches into one from the reads of another.  The four 16-byte
+// pieces of a row lie at piece ^ (row >> 2 & 3): sixteen neighbouring rows of a fragment read then cover all 64 banks.
+// Rows past the end fetch the last row again (their results are not stored); pieces behind column k fetch the last piece again, and the
+// left operand's are zeroed in LDS before the last step is read, so whatever the right operand has there counts nothing.  A tile takes a
+// multiple of four steps; those behind k only keep the ring going.
+constexpr int TK = 64;
+
+template <int WR, int WC, int RB, int CB> struct Tile {
+    static constexpr int WAVES = WR * WC, THREADS = 64 * WAVES, BM = WR * RB * 32, BN = WC * CB * 32;
+    static constexpr int A16 = BM * TK / 16, B16 = BN * TK / 16;             // 16-byte pieces of a stage
+    static constexpr int FA = BM / (16 * WAVES), FB = BN / (16 * WAVES);     // fetches of a wave for a stage
+};
+
+// s_waitcnt vmcnt(n), the other counters left alone
+template <int n> __device__ __forceinline__ void wait_fetches() { __builtin_amdgcn_s_waitcnt(0x0f70 | (n & 15) | (n >> 4) << 14); }
+
+template <class T, int WR, int WC, int RB, int CB>
+__global__ __launch_bounds__(64 * WR * WC) void k_product(ProductArgs p, int n_tiles, int total) {
+    using S = Tile<WR, WC, RB, CB>;
+    __shared__ int4v ring0[S::A16 + S::B16], ring1[S::A16 + S::B16], ring2[S::A16 + S::B16], ring3[S::A16 + S::B16];
+    __shared__ float scales[S::BM + 2 * S::BN] __attribute__((aligned(16)));             // a's, b's, bias of the tile
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave / WC, wc = wave % WC, i32 = lane & 31, half = lane >> 5;
+    const int k16 = (int)((p.k + 15) / 16 * 16), tail = k16 % TK / 16;       // pieces of the last step, 0: all four
+    const int steps = (k16 + TK - 1) / TK, steps4 = (steps + 3) & ~3;
+    auto stage = [&](auto j) -> int4v * {
+        constexpr int J = decltype(j)::value;
+        return J == 0 ? ring0 : J == 1 ? ring1 : J == 2 ? ring2 : ring3;
+    };
+
+    const int frow = wave * 16 + (lane >> 2);          // this lane's row among the 16 WAVES rows that one fetch of all waves covers
+    const int fpiece = ((lane & 3) ^ (lane >> 4)) * 16;
+    // where a tile's rows start: a base per operand, and this lane's rows as 32-bit offsets
+    struct Cursor { const int8_t *a, *b; unsigned ra[S::FA], rb[S::FB]; };
+    auto at_tile = [&](int tile) {
+        const int64_t m0 = (int64_t)(tile / n_tiles) * S::BM, n0 = (int64_t)(tile % n_tiles) * S::BN;
+        const int am = (int)(p.m - 1 - m0 < S::BM ? p.m - 1 - m0 : S::BM), bn = (int)(p.n - 1 - n0 < S::BN ? p.n - 1 - n0 : S::BN);
+        Cursor f;
+        f.a = p.a + m0 * p.lda;
+        f.b = p.b + n0 * p.ldb;
+#pragma unroll
+        for (int i = 0; i < S::FA; ++i) {
+            const int r = i * 16 * S::WAVES + frow;
+            f.ra[i] = (unsigned)((r < am ? r : am) * (int)p.lda);
+        }
+#pragma unroll
+        for (int i = 0; i < S::FB; ++i) {
+            const int r = i * 16 * S::WAVES + frow;
+            f.rb[i] = (unsigned)((r < bn ? r : bn) * (int)p.ldb);
+        }
+        return f;
+    };
+    auto fetch_a = [&](auto j, const Cursor &f, int step) {
+        const int at = step * TK + fpiece, kb = at < k16 ? at : k16 - 16;
+#pragma unroll
+        for (int i = 0; i < S::FA; ++i)
+            __builtin_amdgcn_global_load_lds((global_cvoid_t *)(f.a + (f.ra[i] + kb)), (lds_void_t *)(stage(j) + i * 64 * S::WAVES + wave * 64), 16, 0, 0);
+    };
+    auto fetch_b = [&](auto j, const Cursor &f, int step) {
+        const int at = step * TK + fpiece, kb = at < k16 ? at : k16 - 16;
+#pragma unroll
+        for (int i = 0; i < S::FB; ++i)
+            __builtin_amdgcn_global_load_lds((global_cvoid_t *)(f.b + (f.rb[i] + kb)), (lds_void_t *)(stage(j) + S::A16 + i * 64 * S::WAVES + wave * 64), 16, 0, 0);
+    };
+    int16v acc[CB][RB];
+    // everyone's part of the next stage is in LDS, and nobody reads the stage before it any more.  (__syncthreads would also wait for
+    // the fetches of later stages and for the last tile's stores.)
+    auto meet = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // step k from stage j; the fetches of step `fk` of `f` into the stage before it.  (Every step fetches, under no condition, the last
+    // tile's last steps something that nobody reads: so the counts of the waits are the same on every path, for the compiler's own
+    // waits too.)
+    auto multiply = [&](auto j, int k, const Cursor &f, int fk) {
+        constexpr int J = decltype(j)::value;
+        const std::integral_constant<int, (J + 3) & 3> free;
+        int4v af[2][RB], bf[2][CB];
+        auto products = [&](int q) {
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+#pragma unroll
+                for (int r = 0; r < RB; ++r) acc[c][r] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[q][c], af[q][r], acc[c][r], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (k + 1 == steps && tail) {
+            for (int e = threadIdx.x; e < S::BM * 4; e += S::THREADS)
+                if ((e & 3) >= tail) stage(j)[(e & ~3) + ((e & 3) ^ (e >> 4 & 3))] = int4v{0, 0, 0, 0};
+            meet();
+        }
+        fetch_a(free, f, fk);
+        if (k < steps) {
+            // (indexes that the compiler cannot take apart: behind a longer chain of pointers it loses track of which stage a read is from)
+            const int ra = (wr * RB * 32 + i32) * 4, rb = S::A16 + (wc * CB * 32 + i32) * 4;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                int at = (2 * q + half) ^ (i32 >> 2 & 3), pa = ra + at, pb = rb + at;
+                asm("" : "+v"(pa), "+v"(pb));
+#pragma unroll
+                for (int r = 0; r < RB; ++r) af[q][r] = stage(j)[pa + r * 128];
+#pragma unroll
+                for (int c = 0; c < CB; ++c) bf[q][c] = stage(j)[pb + c * 128];
+            }
+            products(0);
+        }
+        fetch_b(free, f, fk);
+        asm("" : "+s"(k));                             // (or the two ifs become one, and the fetch between them is on two paths)
+        if (k < steps) products(1);
+    };
+    const std::integral_constant<int, 0> s0;
+    const std::integral_constant<int, 1> s1;
+    const std::integral_constant<int, 2> s2;
+    const std::integral_constant<int, 3> s3;
+    // consecutive tiles (which share the rows of a) on one XCD
+    int tile = blockIdx.x;
+    if ((gridDim.x & 7) == 0) tile = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (tile >= total) return;
+    Cursor f = at_tile(tile);
+    fetch_a(s0, f, 0); fetch_b(s0, f, 0);
+    fetch_a(s1, f, 1); fetch_b(s1, f, 1);
+    fetch_a(s2, f, 2); fetch_b(s2, f, 2);
+    constexpr int PER_STAGE = S::FA + S::FB;
+    wait_fetches<0>();
+    for (; tile < total; tile += gridDim.x) {
+        const Cursor next = at_tile(tile + (int)gridDim.x < total ? tile + (int)gridDim.x : tile);
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+                acc[c][r] = int16v(0);
+                asm volatile("" : "+v"(acc[c][r]));    // (else the first step gets a copy of the loop of its own)
+            }
+        // four steps; the last three fetches of a tile are the next tile's first three.  A tile's first three stages were waited for
+        // before the last tile's stores were issued: no wait for those here.
+        auto four = [&](auto first, int k) {
+            constexpr bool WAIT = !decltype(first)::value;
+            const bool end = k + 4 == steps4;
+            const int fk = end ? 0 : k + 4;
+            if (WAIT) wait_fetches<2 * PER_STAGE>();
+            meet();
+            multiply(s0, k, f, k + 3);
+            f.a = end ? next.a : f.a;                  // (selects, not a branch)
+            f.b = end ? next.b : f.b;
+#pragma unroll
+            for (int i = 0; i < S::FA; ++i) f.ra[i] = end ? next.ra[i] : f.ra[i];
+#pragma unroll
+            for (int i = 0; i < S::FB; ++i) f.rb[i] = end ? next.rb[i] : f.rb[i];
+            if (WAIT) wait_fetches<2 * PER_STAGE>();
+            meet();
+            multiply(s1, k + 1, f, fk);
+            if (WAIT) wait_fetches<2 * PER_STAGE>();
+            meet();
+            multiply(s2, k + 2, f, fk + 1);
+            wait_fetches<2 * PER_STAGE>();
+            meet();
+            multiply(s3, k + 3, f, fk + 2);
+        };
+        four(std::true_type{}, 0);
+#pragma clang loop unroll(disable)
+        for (int k = 4; k < steps4; k += 4) four(std::false_type{}, k);
+        // Epilogue.  A lane has one row (the operands are swapped) and registers 4 g .. 4 g + 3 columns 8 g + 4 half ..: stored as they lie
+        // that would be 8 or 16 bytes to each of 32 rows.  So 32 rows x 128 bytes at a time go through this wave's 4 KB of stage 3 (which
+        // nobody reads now) and out as whole 128-byte rows (65536 x 2048 x 2048 in bf16: 541 -> 381 us), past the caches (371 -> 350).  The tile's scales and bias come by way of LDS, and before the first store:
+        // loads and stores are counted in one queue, and a load behind a store would wait for it.
+        const int64_t m0 = (int64_t)(tile / n_tiles) * S::BM, n0 = (int64_t)(tile % n_tiles) * S::BN;
+        constexpr int VALUES = S::BM + 2 * S::BN, TURNS = (VALUES + S::THREADS - 1) / S::THREADS;
+        float held[TURNS];
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            const int e = i * S::THREADS + (int)threadIdx.x;
+            held[i] = 0.f;
+            if (e < S::BM) held[i] = p.sa[m0 + e < p.m ? m0 + e : p.m - 1];
+            else if (e < S::BM + S::BN) held[i] = p.sb[n0 + e - S::BM < p.n ? n0 + e - S::BM : p.n - 1];
+            else if (e < VALUES && p.bias) held[i] = p.bias[n0 + e - S::BM - S::BN < p.n ? n0 + e - S::BM - S::BN : p.n - 1];
+        }
+        wait_fetches<0>();                             // (these loads, and with them the next tile's first three stages)
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i)
+            if (i * S::THREADS + (int)threadIdx.x < VALUES) scales[i * S::THREADS + threadIdx.x] = held[i];
+        meet();                                        // (and nobody reads stage 3 any more)
+        const float low = p.relu ? 0.f : -__builtin_huge_valf();
+        constexpr int PER = 128 / (32 * (int)sizeof(T));         // column blocks in 128 bytes: 1 (fp32) or 2
+        constexpr int V = Vec<T>::N;
+        static_assert(CB % PER == 0 && S::A16 + S::B16 >= S::WAVES * 256, "a wave's 4 KB of stage 3");
+        char *mine = reinterpret_cast<char *>(ring3 + wave * 256);
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+            const float sa = scales[wr * RB * 32 + r * 32 + i32];
+#pragma unroll
+            for (int c0 = 0; c0 < CB; c0 += PER) {
+#pragma unroll
+                for (int c = c0; c < c0 + PER; ++c)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        typedef T quad __attribute__((ext_vector_type(4)));
+                        const int n = (wc * CB + c) * 32 + 8 * g + 4 * half;
+                        const float4 sb = *reinterpret_cast<const float4 *>(scales + S::BM + n), bias = *reinterpret_cast<const float4 *>(scales + S::BM + S::BN + n);
+                        const float s4[4] = {sb.x, sb.y, sb.z, sb.w}, b4[4] = {bias.x, bias.y, bias.z, bias.w};
+                        quad y;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float v = (float)acc[c][r][4 * g + i] * sa * s4[i] + b4[i];
+                            y[i] = (T)(v < low ? low : v);
+                        }
+                        const int byte = ((c - c0) * 32 + 8 * g + 4 * half) * (int)sizeof(T);
+                        *reinterpret_cast<quad *>(mine + i32 * 128 + (((byte >> 4) ^ (i32 >> 1 & 7)) << 4) + (byte & 15)) = y;
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = i * 8 + (lane >> 3), piece = lane & 7;
+                    const typename Vec<T>::raw y = *reinterpret_cast<const typename Vec<T>::raw *>(mine + row * 128 + ((piece ^ (row >> 1 & 7)) << 4));
+                    const int64_t m = m0 + (wr * RB + r) * 32 + row, n = n0 + (wc * CB + c0) * 32 + piece * V;
+                    T *dst = reinterpret_cast<T *>(p.y) + m * p.ldy + n;
+                    if (m < p.m && n + V <= p.n) __builtin_nontemporal_store(y, reinterpret_cast<typename Vec<T>::type *>(dst));
+                    else if (m < p.m)
+#pragma unroll
+                        for (int j = 0; j < V - 1; ++j)
+                            if (n + j < p.n) dst[j] = y[j];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
 }
 
-// 128 x 128 tile, 64 bytes of K per step through LDS, four waves of 64 x 64 (2 x 2 v_mfma_i32_32x32x32_i8)
-constexpr int PT = 128, PK = 64, PLD = PK + 16;        // (+16: the 32 rows of a fragment read fall into different banks)
-template <class T> __global__ __launch_bounds__(256) void k_product(ProductArgs p) {
-    __shared__ int8_t As[PT * PLD] __attribute__((aligned(16)));
-    __shared__ int8_t Bs[PT * PLD] __attribute__((aligned(16)));
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1, i32 = lane & 31, half = lane >> 5;
-    const int64_t m0 = (int64_t)blockIdx.y * PT, n0 = (int64_t)blockIdx.x * PT;
-    int16v acc[2][2] = {};
-    for (int64_t k0 = 0; k0 < p.k; k0 += PK) {
-        int4v ra[2], rb[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int e = threadIdx.x + i * 256, row = e >> 2;
-            const int64_t kq = k0 + (e & 3) * 16;
-            ra[i] = rb[i] = int4v{0, 0, 0, 0};
-            if (kq < p.k && m0 + row < p.m) ra[i] = *reinterpret_cast<const int4v *>(p.a + (m0 + row) * p.lda + kq);
-            if (kq < p.k && n0 + row < p.n) rb[i] = *reinterpret_cast<const int4v *>(p.b + (n0 + row) * p.ldb + kq);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int e = threadIdx.x + i * 256, at = (e >> 2) * PLD + (e & 3) * 16;
-            *reinterpret_cast<int4v *>(As + at) = ra[i];
-            *reinterpret_cast<int4v *>(Bs + at) = rb[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int kk = 0; kk < PK; kk += 32) {
-            int4v af[2], bf[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                af[i] = *reinterpret_cast<const int4v *>(As + (wr * 64 + i * 32 + i32) * PLD + kk + half * 16);
-                bf[i] = *reinterpret_cast<const int4v *>(Bs + (wc * 64 + i * 32 + i32) * PLD + kk + half * 16);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(af[i], bf[j], acc[i][j], 0, 0, 0);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t n = n0 + wc * 64 + j * 32 + i32;
-        if (n >= p.n) continue;
-        const float sb = p.sb[n], bias = p.bias ? p.bias[n] : 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t m = m0 + wr * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-                if (m < p.m) put_product<T>(p, m, n, acc[i][j][r], p.sa[m], sb, bias);
-            }
-    }
+template <class T, int WR, int WC, int RB, int CB> static int tiled(const ProductArgs &p, int cus_per, hipStream_t st) {
+    using S = Tile<WR, WC, RB, CB>;
+    const int64_t nt = (p.n + S::BN - 1) / S::BN, total = nt * ((p.m + S::BM - 1) / S::BM);
+    if (p.lda > (1 << 22) || p.ldb > (1 << 22)) return set_err(MNR_E_INVALID, "the pitches of mnr_int8_product are at most 2^22 bytes");
+    if (total >= (1ll << 30)) return set_err(MNR_E_INVALID, "the output of mnr_int8_product is too large (%lld tiles)", (long long)total);
+    const int64_t most = 256ll * cus_per;
+    hipLaunchKernelGGL((k_product<T, WR, WC, RB, CB>), dim3((unsigned)(total < most ? total : most)), dim3(S::THREADS), 0, st, p, (int)nt, (int)total);
+    return check_launch("k_product");
 }
 
 template <class T> static int product(const ProductArgs &p, hipStream_t st) {
-    hipLaunchKernelGGL((k_product<T>), dim3((unsigned)((p.n + PT - 1) / PT), (unsigned)((p.m + PT - 1) / PT)), dim3(256), 0, st, p);
-    return check_launch("k_product");
+    const int64_t big = ((p.m + 255) / 256) * ((p.n + 255) / 256);
+    if (big >= 192) return tiled<T, 2, 4, 4, 2>(p, 1, st);
+    return tiled<T, 2, 2, 2, 2>(p, 2, st);
 }
 
 template <class T>
