@@ -3,7 +3,7 @@
 //   out[r] = scale table[idx[r]]             grad[v] = scale sum_{r : idx[r] = v} dy[r]
 //
 // Bound by HBM.  The lookup reads 16 bytes per lane wherever the row starts.  The gradient sorts the rows by index (row_sort.hip,
-// stable) and walks the sorted order in tiles: a lane group keeps its columns' fp32 sum of the run it is in, and writes it once when
+// stable; the sort's first launch clears the gradient) and walks the sorted order in tiles of 16 rows: a lane group keeps its columns' fp32 sum of the run it is in, and writes it once when
 // the index changes.  A run that crosses tiles leaves one fp32 sum per tile, joined by k_emb_join in tile order.  No atomics: sums
 // are in row order, the same bits every time, and a popular index costs what an unpopular one does.
 #include "row_sort.h"
@@ -33,12 +33,7 @@ __global__ __launch_bounds__(256) void k_emb_fwd(T *__restrict__ out, int64_t ld
     }
 }
 
-constexpr int EMB_TILE = 32, EMB_STEP = 8;             // sorted rows of a tile; rows in flight
-
-__global__ __launch_bounds__(256) void k_emb_zero(uint32_t *__restrict__ p, int64_t words, int tail_halves) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) p[i] = 0;
-    if (tail_halves && blockIdx.x == 0 && threadIdx.x == 0) reinterpret_cast<uint16_t *>(p + words)[0] = 0;
-}
+constexpr int EMB_TILE = 16;                           // sorted rows of a tile: all of them in flight at once (64 registers)
 
 template <class T>
 __device__ __forceinline__ void emb_write(void *grad, int64_t at, float (&v)[Vec<T>::N], int n, float scale, int grad_f32) {
@@ -54,99 +49,170 @@ __device__ __forceinline__ void emb_write(void *grad, int64_t at, float (&v)[Vec
     }
 }
 
+template <class T>
+__device__ __forceinline__ typename Vec<T>::raw load_raw(const T *p, int n) {
+    if (n >= Vec<T>::N) return *reinterpret_cast<const typename Vec<T>::type *>(p);
+    typename Vec<T>::raw x;
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) x[i] = i < n ? p[i] : (T)0.f;
+    return x;
+}
+template <class T>
+__device__ __forceinline__ void store_sum(float *p, const float (&v)[Vec<T>::N], int n) {
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; i += 4) store_part<float>(p + i, reinterpret_cast<const float (&)[4]>(v[i]), n - i);
+}
+
 // `head[t]`: the sum of tile t's first run where that run began in an earlier tile; `tail[t]`: of its last run where that run began in
 // t and goes on behind it
 template <class T, int LPR>
 __global__ __launch_bounds__(256) void k_emb_sum(void *__restrict__ grad, int grad_f32, float *__restrict__ head, float *__restrict__ tail,
                                                  const T *__restrict__ dy, int64_t ldy, const int32_t *__restrict__ keys,
                                                  const int32_t *__restrict__ order, int64_t n, int width, int64_t padding, float scale) {
-    constexpr int V = Vec<T>::N, GROUPS = 256 / LPR;
+    constexpr int V = Vec<T>::N, GROUPS = 256 / LPR, EACH = (EMB_TILE + LPR - 1) / LPR;
     const int64_t tile = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPR, p0 = tile * EMB_TILE;
-    const int c = ((int)blockIdx.y * LPR + (int)(threadIdx.x % LPR)) * V, m = width - c;
-    if (p0 >= n || m <= 0) return;
-    const int64_t p1 = p0 + EMB_TILE < n ? p0 + EMB_TILE : n;
-    int cur = keys[p0];
-    bool first = p0 > 0 && keys[p0 - 1] == cur;        // the run began before this tile
+    const int t = threadIdx.x % LPR, base = (threadIdx.x & 63) - t;
+    const int c = ((int)blockIdx.y * LPR + t) * V, m = width - c;
+    const int live = p0 >= n ? 0 : (n - p0 < EMB_TILE ? (int)(n - p0) : EMB_TILE);
+    // the group's lanes fetch the tile's keys and rows, one or two each, and hand them round
+    int kk[EACH], oo[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int u = e * LPR + t;
+        kk[e] = u < live ? keys[p0 + u] : -1;
+        oo[e] = u < live ? order[p0 + u] : 0;
+    }
+    const int before = live && p0 > 0 ? keys[p0 - 1] : -1, behind = live == EMB_TILE && p0 + EMB_TILE < n ? keys[p0 + EMB_TILE] : -1;
+    typename Vec<T>::raw v[EMB_TILE];
+#pragma unroll
+    for (int u = 0; u < EMB_TILE; ++u) {
+        const int64_t row = __shfl(oo[u / LPR], base + u % LPR);
+        v[u] = load_raw<T>(dy + row * ldy + c, u < live ? m : 0);
+    }
+    int cur = __shfl(kk[0], base);
+    bool first = live && before == cur;                // the run began before this tile
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    for (int64_t p = p0; p < p1; p += EMB_STEP) {
-        float v[EMB_STEP][V];
-        int k[EMB_STEP];
 #pragma unroll
-        for (int u = 0; u < EMB_STEP; ++u) {
-            const bool in = p + u < p1;
-            k[u] = in ? keys[p + u] : cur;
-            load_part<T>(v[u], dy + (in ? (int64_t)order[p + u] : 0) * ldy + c, in ? m : 0);
+    for (int u = 0; u < EMB_TILE; ++u) {
+        const int k = __shfl(kk[u / LPR], base + u % LPR);
+        if (u < live && k != cur) {
+            if (first) store_sum<T>(head + tile * width + c, acc, m);
+            else if (cur != padding && m > 0) emb_write<T>(grad, (int64_t)cur * width + c, acc, m, scale, grad_f32);
+            first = false;
+            cur = k;
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = 0.f;
         }
 #pragma unroll
-        for (int u = 0; u < EMB_STEP; ++u) {
-            if (p + u >= p1) break;
-            if (k[u] != cur) {
-                if (first) store_part<float>(head + tile * width + c, reinterpret_cast<float (&)[4]>(acc[0]), m);
-                if constexpr (V == 8) { if (first) store_part<float>(head + tile * width + c + 4, reinterpret_cast<float (&)[4]>(acc[4]), m - 4); }
-                if (!first && cur != padding) emb_write<T>(grad, (int64_t)cur * width + c, acc, m, scale, grad_f32);
-                first = false;
-                cur = k[u];
-#pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] = 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] += v[u][i];
-        }
+        for (int i = 0; i < V; ++i) acc[i] += (float)v[u][i];
     }
-    const bool goes_on = p1 < n && keys[p1] == cur;
-    if (first || goes_on) {
-        float *dst = (first ? head : tail) + tile * width + c;
-#pragma unroll
-        for (int i = 0; i < V; i += 4) store_part<float>(dst + i, reinterpret_cast<float (&)[4]>(acc[i]), m - i);
-    } else if (cur != padding) {
-        emb_write<T>(grad, (int64_t)cur * width + c, acc, m, scale, grad_f32);
-    }
+    if (!live || m <= 0) return;
+    if (first || behind == cur) store_sum<T>((first ? head : tail) + tile * width + c, acc, m);
+    else if (cur != padding) emb_write<T>(grad, (int64_t)cur * width + c, acc, m, scale, grad_f32);
 }
 
-// The tile in which a run begins that goes on behind it owns the run: tail[t] + head[t + 1] + ... + head[the tile of its end]
+// The tile in which a run begins that goes on behind it owns the run: tail[t] + head[t + 1] + ... + head[the tile of its end].  A
+// workgroup looks at 16 tiles; a run of up to EMB_SHORT more tiles is joined by one wave, a longer one by the whole workgroup.
+constexpr int EMB_JOIN = 16, EMB_SHORT = 16;
+
+// head[u0], head[u0 + step] ... up to head[last], added to acc
+template <class T>
+__device__ __forceinline__ void emb_add_heads(float (&acc)[Vec<T>::N], const float *head, int64_t u0, int64_t step, int64_t last, int width, int c, int m) {
+#pragma unroll 4
+    for (int64_t u = u0; u <= last; u += step)
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; i += 4) {
+            float v[4];
+            load_part<float>(v, head + u * width + c + i, m - i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i + j] += v[j];
+        }
+}
+
 template <class T, int LPR>
 __global__ __launch_bounds__(256) void k_emb_join(void *__restrict__ grad, int grad_f32, const float *__restrict__ head,
                                                   const float *__restrict__ tail, const int32_t *__restrict__ keys, int64_t n, int width,
                                                   int64_t padding, float scale) {
-    constexpr int V = Vec<T>::N, PH = 256 / LPR;
-    __shared__ float lds[PH > 1 ? PH : 1][LPR * V];
-    const int lane = threadIdx.x % LPR, ph = threadIdx.x / LPR;
+    constexpr int V = Vec<T>::N, PH = 256 / LPR, WPH = 64 / LPR;
+    __shared__ float lds[PH][LPR * V];
+    __shared__ int owner[EMB_JOIN], spans[EMB_JOIN], longer[EMB_JOIN], n_long;
+    const int lane = threadIdx.x % LPR, ph = threadIdx.x / LPR, wave = threadIdx.x >> 6, wph = (threadIdx.x & 63) / LPR;
     const int c = ((int)blockIdx.y * LPR + lane) * V, m = width - c;
-    for (int64_t t = blockIdx.x; (t + 1) * EMB_TILE < n; t += gridDim.x) {
-        const int64_t p0 = t * EMB_TILE, p1 = p0 + EMB_TILE;
-        const int k = keys[p1 - 1];
-        if (keys[p1] != k || k == padding || (p0 > 0 && keys[p0] == k && keys[p0 - 1] == k)) continue;      // (the whole workgroup alike)
-        int64_t lo = p1, hi = n;                       // first place behind the run
-        while (lo < hi) {
-            const int64_t mid = (lo + hi) >> 1;
-            if (keys[mid] == k) lo = mid + 1; else hi = mid;
-        }
-        const int64_t last = (lo - 1) / EMB_TILE;
-        float acc[V], v[4];
-#pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            load_part<float>(v, tail + t * width + c + i, ph == 0 ? m - i : 0);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i + j] = v[j];
-        }
-        for (int64_t u = t + 1 + ph; u <= last; u += PH)
-#pragma unroll
-            for (int i = 0; i < V; i += 4) {
-                load_part<float>(v, head + u * width + c + i, m - i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i + j] += v[j];
+    const int64_t tiles = (n + EMB_TILE - 1) / EMB_TILE;
+    for (int64_t b0 = (int64_t)blockIdx.x * EMB_JOIN; b0 < tiles - 1; b0 += (int64_t)gridDim.x * EMB_JOIN) {
+        __syncthreads();                               // the last round's lists have been read
+        if (threadIdx.x == 0) n_long = 0;
+        if (threadIdx.x < EMB_JOIN) {
+            // tile t owns a run if its last key goes on behind it and did not fill it from before its beginning
+            const int64_t t = b0 + threadIdx.x, p1 = (t + 1) * EMB_TILE;
+            int k = -1;
+            if (p1 < n) {
+                const int64_t p0 = t * EMB_TILE;
+                k = keys[p1 - 1];
+                if (keys[p1] != k || k == padding || (p0 > 0 && keys[p0] == k && keys[p0 - 1] == k)) k = -1;
             }
-        __syncthreads();                               // the last run's sums have been read
-#pragma unroll
-        for (int i = 0; i < V; ++i) lds[ph][lane * V + i] = acc[i];
+            owner[threadIdx.x] = k;
+        }
         __syncthreads();
-        if (ph == 0) {
-            for (int q = 1; q < PH; ++q)
+        for (int o = wave; o < EMB_JOIN; o += 4) {
+            const int k = owner[o];
+            if (k < 0) continue;
+            // the run's last tile: the first tile from t + 1 on that the run does not leave (lane i looks at tile t + 1 + i)
+            const int64_t t = b0 + o, mark = (t + 2 + (threadIdx.x & 63)) * EMB_TILE;
+            const uint64_t leaves = __ballot(mark >= n || keys[mark < n ? mark : n - 1] != k);
+            const int more = leaves ? __ffsll((unsigned long long)leaves) : 65;          // tiles behind t, 65: more than 64
+            if (more > EMB_SHORT) {
+                if ((threadIdx.x & 63) == 0) longer[atomicAdd(&n_long, 1)] = o;
+                if ((threadIdx.x & 63) == 0) spans[o] = leaves ? more : 0;
+                continue;
+            }
+            float acc[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] += lds[q][lane * V + i];
-            if (m > 0) emb_write<T>(grad, (int64_t)k * width + c, acc, m, scale, grad_f32);
+            for (int i = 0; i < V; ++i) acc[i] = 0.f;
+            if (wph == 0) emb_add_heads<T>(acc, tail, t, 1, t, width, c, m);
+            emb_add_heads<T>(acc, head, t + 1 + wph, WPH, t + more, width, c, m);
+            // phases of this wave in order (no other wave touches these rows of lds)
+            wave_sync();
+#pragma unroll
+            for (int i = 0; i < V; ++i) lds[ph][lane * V + i] = acc[i];
+            wave_sync();
+            if (wph == 0 && m > 0) {
+                for (int q = 1; q < WPH; ++q)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[i] += lds[ph + q][lane * V + i];
+                emb_write<T>(grad, (int64_t)k * width + c, acc, m, scale, grad_f32);
+            }
+        }
+        __syncthreads();
+        for (int l = 0; l < n_long; ++l) {             // (in any order: every run is its own row)
+            const int o = longer[l], k = owner[o];
+            const int64_t t = b0 + o;
+            int64_t last = t + spans[o];
+            if (spans[o] == 0) {                       // first place behind the run
+                int64_t lo = (t + 2) * EMB_TILE, hi = n;
+                while (lo < hi) {
+                    const int64_t mid = (lo + hi) >> 1;
+                    if (keys[mid] == k) lo = mid + 1; else hi = mid;
+                }
+                last = (lo - 1) / EMB_TILE;
+            }
+            float acc[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = 0.f;
+            if (ph == 0) emb_add_heads<T>(acc, tail, t, 1, t, width, c, m);
+            emb_add_heads<T>(acc, head, t + 1 + ph, PH, last, width, c, m);
+            __syncthreads();                           // the last run's sums have been read
+#pragma unroll
+            for (int i = 0; i < V; ++i) lds[ph][lane * V + i] = acc[i];
+            __syncthreads();
+            if (ph == 0 && m > 0) {
+                for (int q = 1; q < PH; ++q)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[i] += lds[q][lane * V + i];
+                emb_write<T>(grad, (int64_t)k * width + c, acc, m, scale, grad_f32);
+            }
         }
     }
 }
@@ -176,26 +242,23 @@ static int64_t emb_tiles(int64_t n) { return (n + EMB_TILE - 1) / EMB_TILE; }
 template <class T>
 static int emb_backward(void *grad, int grad_f32, const void *dy, int64_t ldy, int width, const KeySource &src, int64_t rows, int64_t padding,
                         float scale, char *ws, hipStream_t st) {
-    const int64_t words = src.n_keys * width * (grad_f32 ? 4 : (int64_t)sizeof(T)) / 4;
-    const int64_t zb = (words + 1023) / 1024;
-    hipLaunchKernelGGL(k_emb_zero, dim3((unsigned)(zb < 1 ? 1 : (zb > 4096 ? 4096 : zb))), dim3(256), 0, st, (uint32_t *)grad, words,
-                       !grad_f32 && sizeof(T) == 2 && (src.n_keys * width) % 2 ? 1 : 0);
-    int rc = check_launch("k_emb_zero");
-    if (rc != MNR_OK || rows == 0) return rc;
+    const int64_t halves = src.n_keys * width * (grad_f32 ? 2 : (int64_t)sizeof(T) / 2);
+    const SortExtras clear{(uint32_t *)grad, halves / 2, (int)(halves % 2), nullptr};
+    if (rows == 0) return clear_words(clear, st);
     const int64_t tiles = emb_tiles(rows);
     int32_t *order = reinterpret_cast<int32_t *>(ws), *keys = order + rows;
     float *head = reinterpret_cast<float *>(keys + rows), *tail = head + tiles * width;
-    rc = sort_rows(src, rows, order, keys, tail + tiles * width, st);
+    const int rc = sort_rows(src, rows, order, keys, tail + tiles * width, clear, st);
     if (rc != MNR_OK) return rc;
     return emb_lanes(width, Vec<T>::N, [&](auto lpr) {
         constexpr int L = lpr;
         const unsigned gy = (unsigned)((width + L * Vec<T>::N - 1) / (L * Vec<T>::N));
-        const int64_t per = 256 / L;
+        const int64_t per = 256 / L, joins = (tiles - 1 + EMB_JOIN - 1) / EMB_JOIN;
         hipLaunchKernelGGL((k_emb_sum<T, L>), dim3((unsigned)((tiles + per - 1) / per), gy), dim3(256), 0, st, grad, grad_f32, head, tail, (const T *)dy,
                            ldy, keys, order, rows, width, padding, scale);
         if (tiles > 1)
-            hipLaunchKernelGGL((k_emb_join<T, L>), dim3((unsigned)(tiles - 1 < 65536 ? tiles - 1 : 65536), gy), dim3(256), 0, st, grad, grad_f32, head, tail, keys, rows, width,
-                               padding, scale);
+            hipLaunchKernelGGL((k_emb_join<T, L>), dim3((unsigned)(joins < 65536 ? joins : 65536), gy), dim3(256), 0, st, grad, grad_f32, head, tail, keys,
+                               rows, width, padding, scale);
         return check_launch("k_emb_sum / k_emb_join");
     });
 }

@@ -334,16 +334,9 @@ __global__ __launch_bounds__(256) void k_gate_bwd(T *__restrict__ dx, int64_t ld
     }
 }
 
-// offsets[c] = rows of the cells below c: first place in the sorted keys that is not below c
-__global__ __launch_bounds__(256) void k_gate_offsets(int32_t *__restrict__ offsets, const int32_t *__restrict__ keys, int64_t n, int n_cells) {
+__global__ void k_gate_no_offsets(int32_t *__restrict__ offsets, int n) {
     const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c > n_cells) return;
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < c) lo = mid + 1; else hi = mid;
-    }
-    offsets[c] = (int32_t)lo;
+    if (c < n) offsets[c] = 0;
 }
 
 // lanes and cells per lane for n cells: the fewest lanes at up to 8 (above 512 cells 16) values each
@@ -442,11 +435,10 @@ extern "C" int mnr_gate_dispatch(int32_t *order_dev, int32_t *offsets_dev, const
     MNR_REQUIRE(slots == 0 || (workspace_dev && workspace_bytes >= mnr_gate_dispatch_workspace_bytes(slots, n_cells)),
                 "mnr_gate_dispatch needs %zu bytes of workspace", mnr_gate_dispatch_workspace_bytes(slots, n_cells));
     hipStream_t st = as_stream(stream);
-    int32_t *keys = reinterpret_cast<int32_t *>(workspace_dev);
-    if (slots) {
-        const int rc = sort_rows(KeySource{cells_dev, MNR_I32, 1, n_cells}, slots, order_dev, keys, keys + slots, st);
-        if (rc != MNR_OK) return rc;
+    if (slots == 0) {
+        hipLaunchKernelGGL(k_gate_no_offsets, dim3((n_cells + 256) / 256), dim3(256), 0, st, offsets_dev, n_cells + 1);
+        return check_launch("k_gate_no_offsets");
     }
-    hipLaunchKernelGGL(k_gate_offsets, dim3((n_cells + 256) / 256), dim3(256), 0, st, offsets_dev, keys, slots, n_cells);
-    return check_launch("k_gate_offsets");
+    int32_t *keys = reinterpret_cast<int32_t *>(workspace_dev);
+    return sort_rows(KeySource{cells_dev, MNR_I32, 1, n_cells}, slots, order_dev, keys, keys + slots, SortExtras{nullptr, 0, 0, offsets_dev}, st);
 }

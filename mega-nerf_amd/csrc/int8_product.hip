@@ -302,6 +302,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_product(ProductArgs p, int n_t
                         const int byte = ((c - c0) * 32 + 8 * g + 4 * half) * (int)sizeof(T);
                         *reinterpret_cast<quad *>(mine + i32 * 128 + (((byte >> 4) ^ (i32 >> 1 & 7)) << 4) + (byte & 15)) = y;
                     }
+                wave_sync();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = i * 8 + (lane >> 3), piece = lane & 7;
@@ -314,6 +315,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_product(ProductArgs p, int n_t
                         for (int j = 0; j < V - 1; ++j)
                             if (n + j < p.n) dst[j] = y[j];
                 }
+                wave_sync();
                 __builtin_amdgcn_sched_barrier(0);
             }
         }

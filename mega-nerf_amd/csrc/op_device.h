@@ -83,6 +83,12 @@ __device__ __forceinline__ void load_any_part(float (&v)[V], const void *p, int6
     }
 }
 
+// orders LDS accesses between the lanes of one wave (its LDS operations run in order; this keeps the compiler's order too)
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---- reductions over groups of LANES (power of two) consecutive lanes; every lane gets the result -------------------------------
 // Steps 1, 2, 4, 8 are DPP moves inside a row of 16 lanes (quad permutes, half mirror, mirror: after each step the lanes of a
 // sub-group agree, so a mirror is as good as an exchange); 16 and 32 are gfx950's permlane swaps.  No LDS traffic.

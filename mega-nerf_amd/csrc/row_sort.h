@@ -29,7 +29,15 @@ inline bool key_type_ok(int t) { return t == MNR_I32 || t == MNR_I64 || t == MNR
 
 // bytes of scratch for n keys of [0, n_keys] (whole numbers below 2^31)
 size_t sort_rows_bytes(int64_t n, int64_t n_keys);
-// order[p] = row of the p-th smallest (key, row), keys_out[p] = its key
-int sort_rows(const KeySource &src, int64_t n, int32_t *order, int32_t *keys_out, void *ws, hipStream_t st);
+// What else the sort's launches do.  zero: memory that its first launch clears with the workgroups it has to spare (`words` words and
+// then `half` 16-bit words); offsets (NULL: not wanted): [n_keys + 1], first place of every key, rows with key n_keys left out.
+struct SortExtras {
+    uint32_t *zero;  int64_t words;  int half;
+    int32_t *offsets;
+};
+// order[p] = row of the p-th smallest (key, row), keys_out[p] = its key; n >= 1
+int sort_rows(const KeySource &src, int64_t n, int32_t *order, int32_t *keys_out, void *ws, const SortExtras &x, hipStream_t st);
+// x.zero alone (no rows to sort)
+int clear_words(const SortExtras &x, hipStream_t st);
 
 }  // namespace mnr

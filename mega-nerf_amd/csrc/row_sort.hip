@@ -1,16 +1,16 @@
-// row_sort.hip -- stable sort of rows by a small integer key: counting passes over digits of at most 8 bits, lowest first.
+// row_sort.hip -- stable sort of rows by a small integer key: counting passes over digits of at most 11 bits, lowest first.
 //
 // A pass puts row i at  base[digit] + (rows of earlier workgroups with that digit) + (earlier rows of this workgroup with it):
 // k_sort_count counts digits per workgroup, k_sort_scan turns the counts into positions, k_sort_place ranks and writes.  Inside a
 // wave a lane's rank is the number of lower lanes with its digit, from one ballot per bit.  Counts are whole numbers, so the order
-// does not depend on which workgroup ran first; keys of b bits take ceil(b / 8) passes of equal width.  Up to 4096 rows one workgroup
-// does all passes in LDS (one launch).  Traffic is 8 bytes a row and pass each way; at the sizes here (200 K rows) the passes cost
-// their launches, not their bytes.
+// does not depend on which workgroup ran first.  Keys of b bits take ceil(b / 11) passes of equal width: 2048 counters a wave are 32 KB of
+// LDS, and 2000 images sort in one pass (3 launches; two passes of 8 bits took 52 us for 196608 rows).  Up to 4096 rows one workgroup
+// does all passes in LDS (one launch).  At the sizes here the passes cost their launches and the ranking, not their bytes.
 #include "row_sort.h"
 
 namespace mnr {
 
-constexpr int SORT_BLOCK = 256, SORT_ITEMS = 16, SORT_TILE = SORT_BLOCK * SORT_ITEMS, SORT_SMALL = 4096;
+constexpr int SORT_SMALL = 4096, SORT_MAX_BITS = 11, SORT_MAX_DIGITS = 1 << SORT_MAX_BITS;
 
 // lanes of this wave with the same digit as this lane (only lanes with `live` take part)
 __device__ __forceinline__ uint64_t same_digit(int digit, int bits, bool live) {
@@ -32,8 +32,38 @@ __device__ __forceinline__ int take_place(int *counter, int digit, int bits, boo
     return at + __popcll(m & ((1ull << lane) - 1));
 }
 
+// sum of v over this and lower lanes
+__device__ __forceinline__ int scan_wave(int v) {
+    const int lane = threadIdx.x & 63;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+__device__ __forceinline__ void clear_part(const SortExtras &x, int64_t worker, int64_t workers) {
+    for (int64_t i = worker; i < x.words; i += workers) x.zero[i] = 0;
+    if (x.half && worker == 0) reinterpret_cast<uint16_t *>(x.zero + x.words)[0] = 0;
+}
+
+// first place in the sorted keys that is not below c
+__device__ __forceinline__ int64_t first_not_below(const int32_t *keys, int64_t n, int64_t c) {
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (keys[mid] < c) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+// workgroup 0 sorts; the others clear
 __global__ __launch_bounds__(512) void k_sort_small(KeySource src, int n, int bits_per, int passes, int32_t *__restrict__ order,
-                                                    int32_t *__restrict__ keys_out) {
+                                                    int32_t *__restrict__ keys_out, SortExtras x) {
+    if (blockIdx.x > 0) {
+        clear_part(x, (int64_t)(blockIdx.x - 1) * 512 + threadIdx.x, (int64_t)(gridDim.x - 1) * 512);
+        return;
+    }
     __shared__ int key[2][SORT_SMALL];
     __shared__ uint16_t pos[2][SORT_SMALL];
     __shared__ int count[8][256];
@@ -54,11 +84,7 @@ __global__ __launch_bounds__(512) void k_sort_small(KeySource src, int n, int bi
         int total = 0, sum = 0;
         if (d < 256) {
             for (int w = 0; w < 8; ++w) total += count[w][d];
-            sum = total;
-            for (int o = 1; o < 64; o <<= 1) {
-                const int u = __shfl_up(sum, o);
-                if (lane >= o) sum += u;
-            }
+            sum = scan_wave(total);
             if (lane == 63) wave_total[wave] = sum;
         }
         __syncthreads();
@@ -80,130 +106,170 @@ __global__ __launch_bounds__(512) void k_sort_small(KeySource src, int n, int bi
         }
         __syncthreads();
     }
+    const int last = passes & 1;
     for (int i = threadIdx.x; i < n; i += 512) {
-        order[i] = pos[passes & 1][i];
-        keys_out[i] = key[passes & 1][i];
+        order[i] = pos[last][i];
+        keys_out[i] = key[last][i];
     }
+    if (x.offsets)
+        for (int64_t c = threadIdx.x; c <= src.n_keys; c += 512) x.offsets[c] = (int32_t)first_not_below(key[last], n, c);
 }
 
-// hist[digit][workgroup]
-__global__ __launch_bounds__(SORT_BLOCK) void k_sort_count(KeySource src, const int32_t *__restrict__ keys, int64_t n, int shift, int digits,
-                                                           int32_t *__restrict__ hist) {
-    __shared__ int count[256];
-    count[threadIdx.x] = 0;
+// hist[workgroup][digit] for the first `blocks` workgroups; the others clear
+__global__ __launch_bounds__(256) void k_sort_count(KeySource src, const int32_t *__restrict__ keys, int64_t n, int per_block, int blocks, int shift,
+                                                    int digits, int32_t *__restrict__ hist, SortExtras x) {
+    if ((int)blockIdx.x >= blocks) {
+        clear_part(x, (int64_t)(blockIdx.x - blocks) * 256 + threadIdx.x, (int64_t)(gridDim.x - blocks) * 256);
+        return;
+    }
+    __shared__ int count[SORT_MAX_DIGITS];
+    for (int d = threadIdx.x; d < digits; d += 256) count[d] = 0;
     __syncthreads();
-    const int64_t b0 = (int64_t)blockIdx.x * SORT_TILE;
+    const int64_t b0 = (int64_t)blockIdx.x * per_block, b1 = b0 + per_block < n ? b0 + per_block : n;
 #pragma unroll 4
-    for (int j = 0; j < SORT_ITEMS; ++j) {
-        const int64_t i = b0 + j * SORT_BLOCK + threadIdx.x;
-        if (i < n) atomicAdd(&count[((keys ? keys[i] : src(i)) >> shift) & (digits - 1)], 1);
-    }
+    for (int64_t i = b0 + threadIdx.x; i < b1; i += 256) atomicAdd(&count[((keys ? keys[i] : src(i)) >> shift) & (digits - 1)], 1);
     __syncthreads();
-    if ((int)threadIdx.x < digits) hist[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = count[threadIdx.x];
+    for (int d = threadIdx.x; d < digits; d += 256) hist[(int64_t)blockIdx.x * digits + d] = count[d];
 }
 
-// one workgroup per digit: its counts -> rows of that digit in earlier workgroups; total[digit]
-__global__ __launch_bounds__(256) void k_sort_scan(int32_t *__restrict__ hist, int blocks, int32_t *__restrict__ total) {
-    __shared__ int part[4];
-    int32_t *row = hist + (int64_t)blockIdx.x * blocks;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int run = 0;
-    for (int b0 = 0; b0 < blocks; b0 += 256) {
-        const int b = b0 + threadIdx.x, v = b < blocks ? row[b] : 0;
-        int sum = v;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(sum, o);
-            if (lane >= o) sum += u;
-        }
-        __syncthreads();
-        if (lane == 63) part[wave] = sum;
-        __syncthreads();
-        int before = run;
-        for (int w = 0; w < wave; ++w) before += part[w];
-        if (b < blocks) row[b] = before + sum - v;
-        run += part[0] + part[1] + part[2] + part[3];
-    }
-    if (threadIdx.x == 0) total[blockIdx.x] = run;
-}
-
-__global__ __launch_bounds__(SORT_BLOCK) void k_sort_place(KeySource src, const int32_t *__restrict__ keys, const int32_t *__restrict__ rows,
-                                                           int64_t n, int shift, int bits, const int32_t *__restrict__ hist,
-                                                           const int32_t *__restrict__ total, int32_t *__restrict__ keys_out,
-                                                           int32_t *__restrict__ rows_out) {
-    __shared__ int count[4][256];
-    __shared__ int part[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digits = 1 << bits, mask = digits - 1;
-    for (int d = threadIdx.x; d < 4 * 256; d += SORT_BLOCK) (&count[0][0])[d] = 0;
-    __syncthreads();
-    const int64_t i0 = (int64_t)blockIdx.x * SORT_TILE + wave * (SORT_TILE / 4) + lane;
-    int k[SORT_ITEMS];
-#pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j) {
-        const int64_t i = i0 + j * 64;
-        k[j] = i < n ? (keys ? keys[i] : src(i)) : 0;
-        if (i < n) atomicAdd(&count[wave][(k[j] >> shift) & mask], 1);
-    }
-    const int d = threadIdx.x, t = d < digits ? total[d] : 0;
-    int sum = t;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(sum, o);
-        if (lane >= o) sum += u;
-    }
-    if (lane == 63) part[wave] = sum;
-    __syncthreads();
+// 64 digits x 16 segments of workgroups per workgroup: counts -> rows of that digit in earlier workgroups; total[digit]
+__global__ __launch_bounds__(1024) void k_sort_scan(int32_t *__restrict__ hist, int blocks, int digits, int32_t *__restrict__ total) {
+    __shared__ int part[16][64];
+    const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
+    const int per = (blocks + 15) / 16, b0 = seg * per, b1 = min(blocks, b0 + per);
+    int sum = 0;
     if (d < digits) {
-        int at = sum - t + hist[(int64_t)d * gridDim.x + blockIdx.x];
-        for (int w = 0; w < wave; ++w) at += part[w];
-        for (int w = 0; w < 4; ++w) {
-            const int c = count[w][d];
-            count[w][d] = at;
-            at += c;
+#pragma unroll 4
+        for (int b = b0; b < b1; ++b) sum += hist[(int64_t)b * digits + d];
+    }
+    part[seg][lane] = sum;
+    __syncthreads();
+    if (d >= digits) return;
+    int at = 0;
+    for (int s = 0; s < seg; ++s) at += part[s][lane];
+    if (seg == 15) total[d] = at + sum;
+#pragma unroll 4
+    for (int b = b0; b < b1; ++b) {
+        const int c = hist[(int64_t)b * digits + d];
+        hist[(int64_t)b * digits + d] = at;
+        at += c;
+    }
+}
+
+__global__ __launch_bounds__(256) void k_sort_place(KeySource src, const int32_t *__restrict__ keys, const int32_t *__restrict__ rows, int64_t n,
+                                                    int per_block, int shift, int bits, const int32_t *__restrict__ hist,
+                                                    const int32_t *__restrict__ total, int32_t *__restrict__ keys_out,
+                                                    int32_t *__restrict__ rows_out, int32_t *__restrict__ offsets) {
+    extern __shared__ int count[];                     // [4][digits], 4 wave totals
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digits = 1 << bits, mask = digits - 1;
+    int *part = count + 4 * digits;
+    for (int d = threadIdx.x; d < 4 * digits; d += 256) count[d] = 0;
+    __syncthreads();
+    int *mine = count + wave * digits;
+    const int64_t i0 = (int64_t)blockIdx.x * per_block + wave * (per_block / 4), end = i0 + per_block / 4 < n ? i0 + per_block / 4 : n;
+#pragma unroll 4
+    for (int64_t i = i0 + lane; i < end; i += 64) atomicAdd(mine + (((keys ? keys[i] : src(i)) >> shift) & mask), 1);
+    // the digits' bases: a thread sums up its digits / 256 (at least one) neighbours, the workgroup scans the sums
+    const int per = digits >= 256 ? digits / 256 : 1, d0 = threadIdx.x * per;
+    int t[SORT_MAX_DIGITS / 256], sum = 0;
+#pragma unroll
+    for (int j = 0; j < SORT_MAX_DIGITS / 256; ++j) {
+        t[j] = j < per && d0 + j < digits ? total[d0 + j] : 0;
+        sum += t[j];
+    }
+    const int upto = scan_wave(sum);
+    if (lane == 63) part[wave] = upto;
+    __syncthreads();
+    int base = upto - sum;
+    for (int w = 0; w < wave; ++w) base += part[w];
+#pragma unroll
+    for (int j = 0; j < SORT_MAX_DIGITS / 256; ++j) {
+        const int d = d0 + j;
+        if (j < per && d < digits) {
+            if (offsets && blockIdx.x == 0 && d <= src.n_keys) offsets[d] = base;
+            int at = base + hist[(int64_t)blockIdx.x * digits + d];
+            for (int w = 0; w < 4; ++w) {
+                const int c = count[w * digits + d];
+                count[w * digits + d] = at;
+                at += c;
+            }
+            base += t[j];
         }
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j) {
-        const int64_t i = i0 + j * 64;
-        const bool live = i < n;
-        const int at = take_place(count[wave], (k[j] >> shift) & mask, bits, live);
+    for (int64_t i = i0; i < i0 + per_block / 4; i += 64) {
+        const bool live = i + lane < end;
+        const int k = live ? (keys ? keys[i + lane] : src(i + lane)) : 0;
+        const int at = take_place(mine, (k >> shift) & mask, bits, live);
         if (live) {
-            keys_out[at] = k[j];
-            rows_out[at] = rows ? rows[i] : (int32_t)i;
+            keys_out[at] = k;
+            rows_out[at] = rows ? rows[i + lane] : (int32_t)(i + lane);
         }
     }
 }
+
+__global__ __launch_bounds__(256) void k_sort_offsets(int32_t *__restrict__ offsets, const int32_t *__restrict__ keys, int64_t n, int64_t n_keys) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c <= n_keys) offsets[c] = (int32_t)first_not_below(keys, n, c);
+}
+
+__global__ __launch_bounds__(256) void k_clear(SortExtras x) { clear_part(x, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256); }
 
 static int key_bits(int64_t n_keys) {                  // keys 0 .. n_keys
     int b = 1;
     while (((int64_t)1 << b) <= n_keys) ++b;
     return b;
 }
-static int64_t sort_blocks(int64_t n) { return (n + SORT_TILE - 1) / SORT_TILE; }
-
-size_t sort_rows_bytes(int64_t n, int64_t n_keys) {
-    (void)n_keys;
-    if (n <= SORT_SMALL) return 0;
-    return (size_t)(4 * n + 256 * sort_blocks(n) + 256) * sizeof(int32_t);
+// rows of a workgroup: 1024 while that fills the chip, more once the counters of all workgroups would outgrow the rows
+static int sort_per_block(int64_t n) {
+    int64_t per = 1024;
+    while ((n + per - 1) / per > 1024) per *= 2;
+    return (int)per;
+}
+static int64_t sort_blocks(int64_t n) { return (n + sort_per_block(n) - 1) / sort_per_block(n); }
+static unsigned clear_blocks(const SortExtras &x) {
+    if (!x.words && !x.half) return 0;
+    const int64_t n = (x.words + 2047) / 2048;
+    return (unsigned)(n < 1 ? 1 : (n > 2048 ? 2048 : n));
 }
 
-int sort_rows(const KeySource &src, int64_t n, int32_t *order, int32_t *keys_out, void *ws, hipStream_t st) {
-    const int bits = key_bits(src.n_keys), passes = (bits + 7) / 8, per = (bits + passes - 1) / passes;
+size_t sort_rows_bytes(int64_t n, int64_t n_keys) {
+    if (n <= SORT_SMALL) return 0;
+    const int bits = key_bits(n_keys), passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS, per = (bits + passes - 1) / passes;
+    return (size_t)((passes > 1 ? 4 * n : 0) + (sort_blocks(n) + 1) * ((int64_t)1 << per)) * sizeof(int32_t);
+}
+
+int clear_words(const SortExtras &x, hipStream_t st) {
+    if (!clear_blocks(x)) return MNR_OK;
+    hipLaunchKernelGGL(k_clear, dim3(clear_blocks(x)), dim3(256), 0, st, x);
+    return check_launch("k_clear");
+}
+
+int sort_rows(const KeySource &src, int64_t n, int32_t *order, int32_t *keys_out, void *ws, const SortExtras &x, hipStream_t st) {
+    const int bits = key_bits(src.n_keys);
     if (n <= SORT_SMALL) {
-        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(512), 0, st, src, (int)n, per, passes, order, keys_out);
+        const int passes = (bits + 7) / 8, per = (bits + passes - 1) / passes;
+        hipLaunchKernelGGL(k_sort_small, dim3(1 + clear_blocks(x)), dim3(512), 0, st, src, (int)n, per, passes, order, keys_out, x);
         return check_launch("k_sort_small");
     }
-    const int blocks = (int)sort_blocks(n);
-    int32_t *buf = reinterpret_cast<int32_t *>(ws), *hist = buf + 4 * n, *total = hist + (int64_t)256 * blocks;
+    const int passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS, per = (bits + passes - 1) / passes, digits = 1 << per;
+    const int blocks = (int)sort_blocks(n), rows = sort_per_block(n);
+    int32_t *buf = reinterpret_cast<int32_t *>(ws), *hist = buf + (passes > 1 ? 4 * n : 0), *total = hist + (int64_t)digits * blocks;
     const int32_t *ki = nullptr, *ri = nullptr;
+    SortExtras none = {};
     for (int p = 0; p < passes; ++p) {
         const bool last = p == passes - 1;
         int32_t *ko = last ? keys_out : buf + (p & 1) * 2 * n, *ro = last ? order : ko + n;
-        hipLaunchKernelGGL(k_sort_count, dim3(blocks), dim3(SORT_BLOCK), 0, st, src, ki, n, p * per, 1 << per, hist);
-        hipLaunchKernelGGL(k_sort_scan, dim3(1 << per), dim3(256), 0, st, hist, blocks, total);
-        hipLaunchKernelGGL(k_sort_place, dim3(blocks), dim3(SORT_BLOCK), 0, st, src, ki, ri, n, p * per, per, hist, total, ko, ro);
+        hipLaunchKernelGGL(k_sort_count, dim3(blocks + (p ? 0 : clear_blocks(x))), dim3(256), 0, st, src, ki, n, rows, blocks, p * per, digits, hist,
+                           p ? none : x);
+        hipLaunchKernelGGL(k_sort_scan, dim3((digits + 63) / 64), dim3(1024), 0, st, hist, blocks, digits, total);
+        hipLaunchKernelGGL(k_sort_place, dim3(blocks), dim3(256), (size_t)(4 * digits + 4) * sizeof(int), st, src, ki, ri, n, rows, p * per, per, hist,
+                           total, ko, ro, passes == 1 ? x.offsets : nullptr);
         ki = ko;
         ri = ro;
     }
+    if (x.offsets && passes > 1)
+        hipLaunchKernelGGL(k_sort_offsets, dim3((unsigned)((src.n_keys + 256) / 256)), dim3(256), 0, st, x.offsets, keys_out, n, src.n_keys);
     return check_launch("k_sort_place");
 }
 

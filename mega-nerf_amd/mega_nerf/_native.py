@@ -402,7 +402,7 @@ def element_type(t: torch.Tensor, name: str) -> int:
 
 
 def on_device_of(t: torch.Tensor, other: Optional[torch.Tensor], name: str) -> None:
-    if other is not None and other.device != t.device:
+    if other is not None and other.get_device() != t.get_device():
         raise NativeError('{} is on {}, the input on {}'.format(name, other.device, t.device))
 
 
@@ -422,13 +422,18 @@ def matrix(t: torch.Tensor):
     return t, t.numel() // C_ if C_ else 0, C_, C_
 
 
+# the current stream's handle without building a torch.cuda.Stream object (2.7 us a call: more than the launch it is for)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def launch(t: torch.Tensor, fn, *args) -> None:
     """Call a C entry point on the current stream of the device that ``t`` lives on."""
-    if t.device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(t.device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc:
         check(rc)
 

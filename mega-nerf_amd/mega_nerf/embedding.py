@@ -28,9 +28,9 @@ def embedding_forward(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0
     if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
         raise N.NativeError('table must be [count, width] with a row and a column at least (got {})'.format(tuple(table.shape)))
     idx, icode = _index(idx, table)
-    out = torch.empty(*idx.shape, table.shape[1], dtype=table.dtype, device=table.device)
-    table, count, width, ldt = N.matrix(table.detach())
-    N.launch(table, N.lib().mnr_embedding_forward, out.data_ptr(), width, table.data_ptr(), ldt, count, width, idx.data_ptr(), icode, float(scale),
+    out = table.new_empty(idx.shape + table.shape[1:])
+    table, count, width, ldt = N.matrix(table)
+    N.launch(table, N.lib().mnr_embedding_forward, out.data_ptr(), width, table.data_ptr(), ldt, count, width, idx.data_ptr(), icode, scale,
              idx.numel(), code)
     return out
 
@@ -51,11 +51,11 @@ def embedding_backward(dy: torch.Tensor, idx: torch.Tensor, count: int, scale: f
     if padding_idx is not None and not 0 <= pad < count:
         raise N.NativeError('padding_idx must be a row of the table (got {} of {})'.format(padding_idx, count))
     idx, icode = _index(idx, dy)
-    g, rows, width, ldg = N.matrix(dy.detach())
-    grad = torch.empty(count, width, dtype=dtype, device=dy.device)
+    g, rows, width, ldg = N.matrix(dy)
+    grad = dy.new_empty((count, width), dtype=dtype)
     lib = N.lib()
     size = lib.mnr_embedding_backward_workspace_bytes(rows, count, width)
-    ws = torch.empty(size, dtype=torch.uint8, device=dy.device)
+    ws = dy.new_empty(size, dtype=torch.uint8)
     N.launch(g, lib.mnr_embedding_backward, grad.data_ptr(), N.ELEMENT_TYPES[dtype], g.data_ptr(), ldg, idx.data_ptr(), icode, rows, count, width, pad,
              float(scale), code, ws.data_ptr(), size)
     return grad

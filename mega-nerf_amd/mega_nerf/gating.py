@@ -26,7 +26,7 @@ def _logits(logits: torch.Tensor):
     code = N.element_type(logits, 'logits')
     if logits.dim() < 1 or logits.shape[-1] == 0:
         raise N.NativeError('logits must be [..., cells] with a cell at least (got {})'.format(tuple(logits.shape)))
-    return (code,) + tuple(N.matrix(logits.detach()))
+    return (code,) + tuple(N.matrix(logits))
 
 
 def _mask(mask: Optional[torch.Tensor], logits: torch.Tensor):
@@ -64,10 +64,10 @@ def route_topk_forward(logits: torch.Tensor, k: int, score: str = 'softmax', bia
         if bias.dtype != torch.float32 or bias.shape != (n,):
             raise N.NativeError('bias must be float32 [{}] (got {} {})'.format(n, bias.dtype, tuple(bias.shape)))
         N.on_device_of(logits, bias, 'bias')
-        bias = bias.detach().contiguous()
+        bias = bias.contiguous()
     shape = logits.shape[:-1] + (int(k),)
-    weights = torch.empty(shape, dtype=torch.float32, device=x.device)
-    cells = torch.empty(shape, dtype=torch.int32, device=x.device)
+    weights = x.new_empty(shape, dtype=torch.float32)
+    cells = x.new_empty(shape, dtype=torch.int32)
     N.launch(x, N.lib().mnr_gate_forward, weights.data_ptr(), cells.data_ptr(), x.data_ptr(), ldl, N.ptr(bias), N.ptr(m), ldm, rows, n, k, sc, n_groups,
              k_groups, group_top, 1 if renormalise else 0, float(scale), code)
     return weights, cells
@@ -87,8 +87,8 @@ def route_topk_backward(dweights: torch.Tensor, logits: torch.Tensor, cells: tor
     N.on_device_of(logits, cells, 'cells')
     N.on_device_of(logits, dweights, 'dweights')
     cells = cells.contiguous()
-    g, _, k, ldg = N.matrix(dweights.detach())
-    dx = torch.empty(logits.shape, dtype=logits.dtype, device=x.device)
+    g, _, k, ldg = N.matrix(dweights)
+    dx = x.new_empty(logits.shape)
     N.launch(x, N.lib().mnr_gate_backward, dx.data_ptr(), n, g.data_ptr(), ldg, x.data_ptr(), ldl, cells.data_ptr(), N.ptr(m), ldm, rows, n, k, sc,
              1 if renormalise else 0, float(scale), code)
     return dx
@@ -128,10 +128,10 @@ def dispatch(cells: torch.Tensor, n_cells: int) -> Tuple[torch.Tensor, torch.Ten
     N.require_device(cells, 'cells')
     cells = cells.contiguous()
     slots = cells.numel()
-    order = torch.empty(slots, dtype=torch.int32, device=cells.device)
-    offsets = torch.empty(max(int(n_cells), 0) + 1, dtype=torch.int32, device=cells.device)
+    order = cells.new_empty(slots)
+    offsets = cells.new_empty(max(int(n_cells), 0) + 1)
     lib = N.lib()
     size = lib.mnr_gate_dispatch_workspace_bytes(slots, n_cells)
-    ws = torch.empty(size, dtype=torch.uint8, device=cells.device)
+    ws = cells.new_empty(size, dtype=torch.uint8)
     N.launch(cells, lib.mnr_gate_dispatch, order.data_ptr(), offsets.data_ptr(), cells.data_ptr(), slots, n_cells, ws.data_ptr(), size)
     return order, offsets

@@ -22,7 +22,7 @@ def _check(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch
         if t is None:
             continue
         wcode = N.element_type(t, name)
-        if t.shape != x.shape[-1:]:
+        if t.dim() != 1 or t.shape[0] != x.shape[-1]:
             raise N.NativeError('{} must have shape {} (got {})'.format(name, tuple(x.shape[-1:]), tuple(t.shape)))
         N.on_device_of(x, t, name)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
@@ -36,15 +36,15 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     bfloat16; ``weight`` / ``bias`` [C] of any of them."""
     code, wcode = _check(x, weight, bias)
     shape = x.shape
-    x, rows, cols, ldx = N.matrix(x.detach())
-    w = weight.detach().contiguous() if weight is not None else None
-    b = bias.detach().contiguous() if bias is not None else None
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
-    at = stats.data_ptr()
-    N.launch(x, N.lib().mnr_layer_norm_forward, y.data_ptr(), cols, at, at + 4 * rows, x.data_ptr(), ldx, N.ptr(w), N.ptr(b), rows, cols, float(eps),
-             code, wcode)
-    return y, stats[0], stats[1]
+    x, rows, cols, ldx = N.matrix(x)
+    w = weight.contiguous() if weight is not None else None
+    b = bias.contiguous() if bias is not None else None
+    y = x.new_empty(shape)
+    mean = x.new_empty(rows, dtype=torch.float32)
+    rstd = x.new_empty(rows, dtype=torch.float32)
+    N.launch(x, N.lib().mnr_layer_norm_forward, y.data_ptr(), cols, mean.data_ptr(), rstd.data_ptr(), x.data_ptr(), ldx, N.ptr(w), N.ptr(b), rows, cols,
+             eps, code, wcode)
+    return y, mean, rstd
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor, rstd: torch.Tensor,
@@ -55,21 +55,21 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise N.NativeError('dy must be like x: {} {} (got {} {})'.format(tuple(x.shape), x.dtype, tuple(dy.shape), dy.dtype))
     N.on_device_of(x, dy, 'dy')
-    x, rows, cols, ldx = N.matrix(x.detach())
-    g, _, _, ldg = N.matrix(dy.detach())
+    x, rows, cols, ldx = N.matrix(x)
+    g, _, _, ldg = N.matrix(dy)
     for t, name in ((mean, 'mean'), (rstd, 'rstd')):
         if t.dtype != torch.float32 or t.numel() != rows:
             raise N.NativeError('{} must be float32 with {} elements, as layer_norm_forward returned it'.format(name, rows))
         N.on_device_of(x, t, name)
-    mean, rstd = mean.detach().contiguous(), rstd.detach().contiguous()
-    w = weight.detach().contiguous() if weight is not None else None
-    dx = torch.empty(dy.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    w = weight.contiguous() if weight is not None else None
+    dx = x.new_empty(dy.shape) if need[0] else None
     wtype = weight.dtype if weight is not None else torch.float32
-    dw = torch.empty(cols, dtype=wtype, device=x.device) if need[1] else None
-    db = torch.empty(cols, dtype=wtype, device=x.device) if need[2] else None
+    dw = x.new_empty(cols, dtype=wtype) if need[1] else None
+    db = x.new_empty(cols, dtype=wtype) if need[2] else None
     lib = N.lib()
     size = lib.mnr_layer_norm_backward_workspace_bytes(rows, cols, code) if need[1] or need[2] else 0
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    ws = x.new_empty(size, dtype=torch.uint8) if size else None
     N.launch(x, lib.mnr_layer_norm_backward, N.ptr(dx), cols, N.ptr(dw), N.ptr(db), g.data_ptr(), ldg, x.data_ptr(), ldx, N.ptr(w), mean.data_ptr(),
              rstd.data_ptr(), rows, cols, code, wcode, N.ptr(ws), size)
     return dx, dw, db

@@ -29,10 +29,10 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     code = N.element_type(x, 'x')
     if x.dim() != 2 or x.shape[1] == 0:
         raise N.NativeError('quantize_rows expects [rows, cols] with a column at least (got {})'.format(tuple(x.shape)))
-    x, rows, cols, ldx = N.matrix(x.detach())
+    x, rows, cols, ldx = N.matrix(x)
     pitch = (cols + _PITCH - 1) // _PITCH * _PITCH
-    values = torch.empty(rows, pitch, dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    values = x.new_empty((rows, pitch), dtype=torch.int8)
+    scale = x.new_empty(rows, dtype=torch.float32)
     N.launch(x, N.lib().mnr_quantize_rows, values.data_ptr(), pitch, scale.data_ptr(), x.data_ptr(), ldx, rows, cols, code)
     return QuantizedRows(values[:, :cols] if pitch > cols else values, scale)
 
@@ -71,15 +71,15 @@ def _product(a, m, k, lda, a_scale, b: QuantizedRows, bias, relu, out_dtype) -> 
         if bias.dtype != torch.float32 or bias.shape != (n,):
             raise N.NativeError('bias must be float32 [{}] (got {} {})'.format(n, bias.dtype, tuple(bias.shape)))
         N.on_device_of(a, bias, 'bias')
-        bias = bias.detach().contiguous()
+        bias = bias.contiguous()
     code = N.ELEMENT_TYPES.get(out_dtype)
     if code is None:
         raise N.NativeError('the output is float32, float16 or bfloat16 (got {})'.format(out_dtype))
     a_scale, b_scale = a_scale.contiguous(), b.scale.contiguous()
-    y = torch.empty(m, n, dtype=out_dtype, device=a.device)
+    y = a.new_empty((m, n), dtype=out_dtype)
     lib = N.lib()
     size = lib.mnr_int8_product_workspace_bytes(m, n, k)
-    ws = torch.empty(size, dtype=torch.uint8, device=a.device) if size else None
+    ws = a.new_empty(size, dtype=torch.uint8) if size else None
     N.launch(a, lib.mnr_int8_product, y.data_ptr(), n, a.data_ptr(), lda, a_scale.data_ptr(), bv.data_ptr(), ldb, b_scale.data_ptr(),
              N.ptr(bias), m, n, k, 1 if relu else 0, code, N.ptr(ws), size)
     return y
