@@ -250,12 +250,15 @@ int mnr_gate_dispatch(int32_t *order_dev, int32_t *offsets_dev, const int32_t *c
 int mnr_quantize_rows(int8_t *values_dev, int64_t pitch, float *scale_dev, const void *x_dev, int64_t ldx, int64_t rows, int64_t cols,
                       int type, void *stream);
 /* y[m][n] = act( a_scale[m] b_scale[n] sum_k a[m][k] b[n][k] + bias[n] ), the sum exact in int32 (k <= 131071); act: 0 none, 1 ReLU.
- * a / b start at a multiple of 16 bytes with pitches that are multiples of 16; where k is no multiple of 16, a's rows (not b's) are
+ * a / b start at a multiple of 16 bytes with pitches that are multiples of 16 below 2^22; where k is no multiple of 16, a's rows (not b's) are
  * zero behind column k, and both can be read up to the next multiple of 16. */
-size_t mnr_int8_product_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int mnr_int8_product(void *y_dev, int64_t ldy, const int8_t *a_dev, int64_t lda, const float *a_scale_dev, const int8_t *b_dev, int64_t ldb,
-                     const float *b_scale_dev, const float *bias_dev, int64_t m, int64_t n, int64_t k, int act, int type,
-                     void *workspace_dev, size_t workspace_bytes, void *stream);
+                     const float *b_scale_dev, const float *bias_dev, int64_t m, int64_t n, int64_t k, int act, int type, void *stream);
+/* A dense layer: mnr_quantize_rows of x [m][k] (x_type) into the workspace, then mnr_int8_product with the weight b [n][k] */
+size_t mnr_int8_linear_workspace_bytes(int64_t m, int64_t k);
+int mnr_int8_linear(void *y_dev, int64_t ldy, const void *x_dev, int64_t ldx, int x_type, const int8_t *b_dev, int64_t ldb,
+                    const float *b_scale_dev, const float *bias_dev, int64_t m, int64_t n, int64_t k, int act, int type,
+                    void *workspace_dev, size_t workspace_bytes, void *stream);
 
 /* ---- wide layers of the layer-by-layer path: tiled GEMM with fused epilogues (csrc/tgemm.hip) and batched weight
  * gradients (csrc/wgrad.hip); what nerf.py:115-160 + autograd get from cuBLAS, for layer widths that are multiples of 256.

@@ -50,14 +50,6 @@ __device__ __forceinline__ void emb_write(void *grad, int64_t at, float (&v)[Vec
 }
 
 template <class T>
-__device__ __forceinline__ typename Vec<T>::raw load_raw(const T *p, int n) {
-    if (n >= Vec<T>::N) return *reinterpret_cast<const typename Vec<T>::type *>(p);
-    typename Vec<T>::raw x;
-#pragma unroll
-    for (int i = 0; i < Vec<T>::N; ++i) x[i] = i < n ? p[i] : (T)0.f;
-    return x;
-}
-template <class T>
 __device__ __forceinline__ void store_sum(float *p, const float (&v)[Vec<T>::N], int n) {
 #pragma unroll
     for (int i = 0; i < Vec<T>::N; i += 4) store_part<float>(p + i, reinterpret_cast<const float (&)[4]>(v[i]), n - i);
@@ -114,13 +106,15 @@ __global__ __launch_bounds__(256) void k_emb_sum(void *__restrict__ grad, int gr
 }
 
 // The tile in which a run begins that goes on behind it owns the run: tail[t] + head[t + 1] + ... + head[the tile of its end].  A
-// workgroup looks at 16 tiles; a run of up to EMB_SHORT more tiles is joined by one wave, a longer one by the whole workgroup.
+// workgroup looks at 16 tiles; a run of up to EMB_SHORT more tiles is joined by one wave, a longer one by the whole workgroup.  Eight
+// lanes share a sum's columns, whatever the width, and the columns are spread over workgroups: so a run over a sixth of 65521 rows
+// (676 tiles of 512 columns) is added up by 8 workgroups in 32 phases each (64 lanes and 4 phases: 77 us).
 constexpr int EMB_JOIN = 16, EMB_SHORT = 16;
 
 // head[u0], head[u0 + step] ... up to head[last], added to acc
 template <class T>
 __device__ __forceinline__ void emb_add_heads(float (&acc)[Vec<T>::N], const float *head, int64_t u0, int64_t step, int64_t last, int width, int c, int m) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t u = u0; u <= last; u += step)
 #pragma unroll
         for (int i = 0; i < Vec<T>::N; i += 4) {
@@ -257,8 +251,8 @@ static int emb_backward(void *grad, int grad_f32, const void *dy, int64_t ldy, i
         hipLaunchKernelGGL((k_emb_sum<T, L>), dim3((unsigned)((tiles + per - 1) / per), gy), dim3(256), 0, st, grad, grad_f32, head, tail, (const T *)dy,
                            ldy, keys, order, rows, width, padding, scale);
         if (tiles > 1)
-            hipLaunchKernelGGL((k_emb_join<T, L>), dim3((unsigned)(joins < 65536 ? joins : 65536), gy), dim3(256), 0, st, grad, grad_f32, head, tail, keys,
-                               rows, width, padding, scale);
+            hipLaunchKernelGGL((k_emb_join<T, 8>), dim3((unsigned)(joins < 65536 ? joins : 65536), (unsigned)((width + 8 * Vec<T>::N - 1) / (8 * Vec<T>::N))),
+                               dim3(256), 0, st, grad, grad_f32, head, tail, keys, rows, width, padding, scale);
         return check_launch("k_emb_sum / k_emb_join");
     });
 }

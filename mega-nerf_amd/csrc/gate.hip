@@ -7,10 +7,16 @@
 //   gradient (cells fixed), g = scale dw:    softmax, renormalised: dx_j = p_j (g_j - sum p g) over the chosen, p = w / scale
 //       softmax: dx_e = s_e (g_e [e chosen] - sum_chosen s g);   sigmoid: dx_j = s_j (1 - s_j) g_j, renormalised p_j (1 - s_j) (g_j - sum p g)
 //
-// Bound by HBM for few cells (a row is read once), by the rounds of arg-max for many.  8 to 64 lanes share a row and keep its
-// selection values in registers; a round is a local scan and a DPP reduction.  Where no score enters a comparison the values are the
-// logits themselves (exact); otherwise they are in 64 bits, so that the choice is the one of the definition.
+// Bound by HBM for few cells (a row is read once), by the instructions of the arg-max rounds for many.  A lane holds up to 32 neighbouring
+// cells in registers, so up to 32 cells need no exchange at all (a thread is a row) and 256 cells 8 lanes: a round is a local maximum, a
+// DPP maximum over the lanes and a ballot that names the lowest lane that has it.  (With 4 cells a lane and 8 lanes a row every
+// instruction served 8 rows instead of 64: 25 cells took 20 us; 8 cells and 32 lanes: 256 cells 122 us.)  Where no score enters a comparison the values are the logits themselves (exact).  Otherwise the
+// scores are formed in fp32 and every decision is checked: a row where two values that a decision kept apart are closer than fp32's
+// error is decided again in 64 bits, by the whole wave, so the choice is always the one of the definition (all rows in 64 bits: 256
+// cells in 8 groups, 65536 rows of bf16 took 266 us).
 // Weights are formed from the logits of the chosen (log-sigmoids for sigmoid), so renormalising never divides by an underflowed sum.
+#include <type_traits>
+
 #include "row_sort.h"
 
 namespace mnr {
@@ -99,146 +105,327 @@ constexpr float GATE_NONE = -__builtin_huge_valf();
 
 __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
 
-// LPR lanes share a row; lane t holds cells t, t + LPR, ... (EPL of them) and slots t, t + LPR, ... (KPL of them)
-template <class T, int LPR, int EPL, class V>
-__global__ __launch_bounds__(256) void k_gate_fwd(float *__restrict__ weights, int32_t *__restrict__ cells, GateArgs a) {
-    constexpr int RPB = 256 / LPR, KPL = (GATE_MAX_K + LPR - 1) / LPR < EPL ? (GATE_MAX_K + LPR - 1) / LPR : EPL;
-    constexpr bool WIDE = sizeof(V) == 8;
-    const V none = (V)GATE_NONE;
-    const int t = threadIdx.x % LPR;
-    const int per_group = a.n / a.n_groups;
-    int group[EPL];
-    if (a.n_groups > 1)
+// this lane's cells e0 .. of a row: the logits of the open ones, GATE_NONE elsewhere
+template <class T, int EPL>
+__device__ __forceinline__ void gate_load(float (&x)[EPL], const GateArgs &a, const T *row, int64_t r, int e0, bool live) {
+    constexpr int N = EPL < Vec<T>::N ? EPL : Vec<T>::N;
+    typedef T part __attribute__((ext_vector_type(N)));
+    typedef part part_at __attribute__((aligned(sizeof(T))));
+    typedef uint8_t bytes __attribute__((ext_vector_type(N)));
+    typedef bytes bytes_at __attribute__((aligned(1)));
+    const int left = live ? a.n - e0 : 0;
+    const uint8_t *open = a.mask + r * a.ldm + e0;
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) group[j] = (j * LPR + t) / per_group;
+    for (int j = 0; j < EPL; j += N) {
+        if (left >= j + N) {
+            const part v = *reinterpret_cast<const part_at *>(row + e0 + j);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[j + i] = (float)v[i];
+            if (a.mask) {
+                const bytes m = *reinterpret_cast<const bytes_at *>(open + j);
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[j + i] = m[i] ? x[j + i] : GATE_NONE;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                x[j + i] = GATE_NONE;
+                if (j + i < left && !(a.mask && !open[j + i])) x[j + i] = (float)row[e0 + j + i];
+            }
+        }
+    }
+}
+
+// the ballot of this lane's group, its lowest lane in bit 0
+template <int LPR> __device__ __forceinline__ uint64_t group_ballot(bool b) {
+    if constexpr (LPR == 1) return b;
+    const uint64_t m = __ballot(b);
+    if constexpr (LPR == 64) return m;
+    return (m >> ((threadIdx.x & 63) / LPR * LPR)) & ((1ull << LPR) - 1);
+}
+template <int LPR> __device__ __forceinline__ float group_max(float x) { return lane_max<LPR>(x); }
+template <int LPR> __device__ __forceinline__ double group_max(double x) {
+    Best<double> b{x, 0};
+    lane_best<LPR>(b);
+    return b.v;
+}
+
+// Takes the largest of the group's values out of v: its value, and on the lane that had it `mine` = its number there, else -1
+template <int LPR, int EPL, class V> __device__ __forceinline__ V take_best(V (&v)[EPL], int &mine) {
+    const V none = (V)GATE_NONE;
+    V high = v[0];
+#pragma unroll
+    for (int j = 1; j < EPL; ++j) high = v[j] > high ? v[j] : high;
+    const V best = group_max<LPR>(high);
+    bool own = best > none;
+    if constexpr (LPR > 1) {
+        const uint64_t who = group_ballot<LPR>(high == best);
+        own = own && (int)(threadIdx.x % LPR) == __ffsll((unsigned long long)who) - 1;
+    }
+    mine = -1;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        const bool hit = own && v[j] == best;
+        v[j] = hit ? none : v[j];
+        mine = hit ? j : mine;
+        own = own && !hit;
+    }
+    return best;
+}
+
+// The two largest of two pairs of (largest, second)
+template <class V> __device__ __forceinline__ void merge_two(V &a1, V &a2, V b1, V b2) {
+    const V low = a1 < b1 ? a1 : b1, high = a1 < b1 ? b1 : a1, second = a2 < b2 ? b2 : a2;
+    a1 = high;
+    a2 = low < second ? second : low;
+}
+template <int STEP, class V> __device__ __forceinline__ void merge_two_step(V &a1, V &a2) {
+    if constexpr (STEP >= 16) {
+        V p1, q1, p2, q2;
+        halves_of<STEP>(a1, p1, q1);
+        halves_of<STEP>(a2, p2, q2);
+        a1 = p1; a2 = p2;
+        merge_two(a1, a2, q1, q2);
+    } else {
+        merge_two(a1, a2, other_of<STEP>(a1), other_of<STEP>(a2));
+    }
+}
+template <int LANES, class V> __device__ __forceinline__ void merge_two_lanes(V &a1, V &a2) {
+    if constexpr (LANES >= 2) merge_two_step<1>(a1, a2);
+    if constexpr (LANES >= 4) merge_two_step<2>(a1, a2);
+    if constexpr (LANES >= 8) merge_two_step<4>(a1, a2);
+    if constexpr (LANES >= 16) merge_two_step<8>(a1, a2);
+    if constexpr (LANES >= 32) merge_two_step<16>(a1, a2);
+    if constexpr (LANES >= 64) merge_two_step<32>(a1, a2);
+}
+template <class V> __device__ __forceinline__ V group_total(V a1, V a2, int top) {
+    return top > 1 && a2 > (V)GATE_NONE ? a1 + a2 : a1;      // (a1 none: none)
+}
+
+// Closes the cells of the groups that are not among the best k_groups.  `near` becomes true where the choice hangs on a difference of at
+// most `margin`.  LANES: a group is the cells of a power of two of whole lanes (one pass for all groups); else any size, group by group.
+template <int LPR, int EPL, bool LANES, class V>
+__device__ __forceinline__ void gate_groups(V (&v)[EPL], const GateArgs &a, V margin, bool &near) {
+    const V none = (V)GATE_NONE;
+    const int t = threadIdx.x % LPR, per_group = a.n / a.n_groups;
+    V last = none;
+    if constexpr (LANES) {
+        const int lanes = per_group / EPL;
+        V a1 = v[0], a2 = none;
+#pragma unroll
+        for (int j = 1; j < EPL; ++j) merge_two(a1, a2, v[j], none);
+        if constexpr (LPR >= 4) { if (lanes >= 2) merge_two_step<1>(a1, a2); }
+        if constexpr (LPR >= 8) { if (lanes >= 4) merge_two_step<2>(a1, a2); }
+        if constexpr (LPR >= 16) { if (lanes >= 8) merge_two_step<4>(a1, a2); }
+        if constexpr (LPR >= 32) { if (lanes >= 16) merge_two_step<8>(a1, a2); }
+        V total[1] = {(t & (lanes - 1)) == 0 ? group_total(a1, a2, a.group_top) : none};         // its first lane holds it
+        bool keep = false;
+        for (int q = 0; q <= a.k_groups && q < a.n_groups; ++q) {
+            int mine;
+            const V best = take_best<LPR, 1>(total, mine);
+            if (q == a.k_groups) near = near || (best > none && last - best <= margin);
+            else {
+                last = best;
+                const uint64_t who = group_ballot<LPR>(mine >= 0);
+                keep = keep || (who && ((__ffsll((unsigned long long)who) - 1) ^ t) < lanes);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) v[j] = keep ? v[j] : none;
+    } else {
+        V total[EPL];                                  // of groups t EPL + j
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) total[j] = none;
+        for (int g = 0; g < a.n_groups; ++g) {
+            V a1 = none, a2 = none;
+            // this lane's cells of group g: from `from` up to `from + per_group`
+            const int from = g * per_group - t * EPL;
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) merge_two(a1, a2, (unsigned)(j - from) < (unsigned)per_group ? v[j] : none, none);
+            merge_two_lanes<LPR>(a1, a2);
+#pragma unroll
+            for (int j = 0; j < EPL; ++j)
+                if (t * EPL + j == g) total[j] = group_total(a1, a2, a.group_top);
+        }
+        uint32_t keep = 0;
+        for (int q = 0; q <= a.k_groups && q < a.n_groups; ++q) {
+            int mine;
+            const V best = take_best<LPR, EPL>(total, mine);
+            if (q == a.k_groups) near = near || (best > none && last - best <= margin);
+            else {
+                last = best;
+                int g = mine;                          // which group that was, for all lanes
+                if constexpr (LPR > 1) {
+                    const uint64_t who = group_ballot<LPR>(mine >= 0);
+                    const int lane = who ? __ffsll((unsigned long long)who) - 1 : 0, its = __shfl(mine, (int)(threadIdx.x & 63) - t + lane);
+                    g = its < 0 ? -1 : lane * EPL + its;
+                }
+                const int from = g < 0 ? EPL : g * per_group - t * EPL;
+#pragma unroll
+                for (int j = 0; j < EPL; ++j)
+                    if ((unsigned)(j - from) < (unsigned)per_group) keep |= 1u << j;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) v[j] = (keep >> j) & 1 ? v[j] : none;
+    }
+}
+
+// Writes the chosen cells to `chosen` [k] (LDS, -1 where there are no more).  `near` as above, over the order of the chosen and the last
+// one's lead over the rest.
+template <int LPR, int EPL, class V>
+__device__ __forceinline__ void gate_choose(V (&v)[EPL], int k, bool check, V margin, bool &near, int *chosen) {
+    const int t = threadIdx.x % LPR;
+    V last = (V)__builtin_huge_valf();
+    for (int s = 0; s < k + (check ? 1 : 0); ++s) {
+        int mine;
+        const V best = take_best<LPR, EPL>(v, mine);
+        if (check) {                                   // (uniform)
+            near = near || (best > (V)GATE_NONE && s > 0 && last - best <= margin);
+            last = best;
+        }
+        if (s < k) {
+            if (mine >= 0) chosen[s] = t * EPL + mine;
+            else if (t == 0 && !(best > (V)GATE_NONE)) chosen[s] = -1;
+        }
+    }
+}
+
+// the choice of row r in 64 bits, by all lanes of the wave, EPL cells each
+template <class T, int EPL> __device__ __forceinline__ void gate_exact(const GateArgs &a, int64_t r, int *chosen) {
+    const int e0 = (int)(threadIdx.x & 63) * EPL;
+    float x[EPL], at = GATE_NONE;
+    gate_load<T, EPL>(x, a, reinterpret_cast<const T *>(a.logits) + r * a.ldl, r, e0, true);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) at = fmaxf(at, x[j]);
+    at = lane_max<64>(at);
+    double v[EPL], total = 0.;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        v[j] = a.sigmoid ? 1. / (1. + exp(-(double)x[j])) : exp((double)x[j] - (double)at);
+        total += v[j];
+    }
+    total = a.sigmoid ? 1. : lane_sum64<64>(total);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        v[j] = v[j] / total;
+        if (a.bias) v[j] += e0 + j < a.n ? (double)a.bias[e0 + j] : 0.;
+        v[j] = x[j] > GATE_NONE ? v[j] : (double)GATE_NONE;
+    }
+    bool done = false;
+    if (a.n_groups > 1) gate_groups<64, EPL, false>(v, a, -1., done);
+    if (!a.bias)
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) v[j] = v[j] > (double)GATE_NONE ? (double)x[j] : (double)GATE_NONE;
+    gate_choose<64, EPL>(v, a.k, false, -1., done, chosen);
+}
+
+// LPR lanes share a row, lane t holds cells t EPL ... and slots t, t + LPR, ...
+template <class T, int LPR, int EPL, bool SCORED, bool LANES>
+__global__ __launch_bounds__(256, SCORED ? 2 : 4) void k_gate_fwd(float *__restrict__ weights, int32_t *__restrict__ cells, GateArgs a) {
+    constexpr int RPB = 256 / LPR, MAX_K = LPR * EPL < GATE_MAX_K ? LPR * EPL : GATE_MAX_K;
+    __shared__ int chosen[RPB][MAX_K + 1];             // (+1: a column's entries fall into different banks)
+    const int t = threadIdx.x % LPR, e0 = t * EPL;
+    int *const mine = chosen[threadIdx.x / LPR];
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
         const int64_t r = r0 + threadIdx.x / LPR;
         const bool live = r < a.rows;
         const T *row = reinterpret_cast<const T *>(a.logits) + r * a.ldl;
-        float x[EPL], high = GATE_NONE, bad = 0.f;
+        float x[EPL], high = GATE_NONE;
+        gate_load<T, EPL>(x, a, row, r, e0, live);
+        bool bad = false;                              // a NaN, or +inf under softmax
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
-            const int e = j * LPR + t;
-            bool open = live && e < a.n;
-            if (open && a.mask) open = a.mask[r * a.ldm + e] != 0;
-            x[j] = open ? (float)row[e] : GATE_NONE;
-            if (!(x[j] < __builtin_huge_valf()) && !(a.sigmoid && x[j] == x[j])) bad = 1.f;       // a NaN, or +inf under softmax
+            bad = bad || !(a.sigmoid ? x[j] <= __builtin_huge_valf() : x[j] < __builtin_huge_valf());
             high = fmaxf(high, x[j]);
         }
-        high = lane_max<LPR>(high);
-        const float at = high > GATE_NONE ? high : 0.f;
-        V v[EPL];                                     // what is compared
-        if constexpr (WIDE) {
-            double total = 0.;
+        if (!a.sigmoid) high = lane_max<LPR>(high);
+        const float at = high > GATE_NONE ? high : 0.f;      // (softmax: what the exponents are relative to)
+        float all = 1.f;                                     // the softmax's sum, where it is needed
+        if (!a.sigmoid && (SCORED || !a.renormalise)) {
+            all = 0.f;
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) {
-                v[j] = a.sigmoid ? 1. / (1. + exp(-(double)x[j])) : exp((double)x[j] - (double)at);
-                total += v[j];
-            }
-            total = a.sigmoid ? 1. : lane_sum64<LPR>(total);
-#pragma unroll
-            for (int j = 0; j < EPL; ++j) {
-                v[j] = x[j] > GATE_NONE ? v[j] / total : none;
-                if (a.bias && x[j] > GATE_NONE) {
-                    v[j] += (double)a.bias[j * LPR + t];
-                    if (v[j] != v[j]) bad = 1.f;
-                }
-            }
-        } else {
+            for (int j = 0; j < EPL; ++j) all += expf(x[j] - at);
+            all = lane_sum<LPR>(all);
+        }
+        wave_sync();                                         // the last row's list has been read
+        if constexpr (!SCORED) {
+            float v[EPL];
 #pragma unroll
             for (int j = 0; j < EPL; ++j) v[j] = x[j];
-        }
-        bad = lane_max<LPR>(bad);
-        if (a.n_groups > 1) {
-            V total[EPL];                             // of groups t, t + LPR, ...
+            bool exact = false;
+            if (a.n_groups > 1) gate_groups<LPR, EPL, LANES>(v, a, -1.f, exact);
+            bad = group_ballot<LPR>(bad) != 0;
+            gate_choose<LPR, EPL>(v, a.k, false, -1.f, exact, mine);
+        } else {
+            bool near = false;
+            const float each = all > 0.f ? 1.f / all : 0.f;
+            float v[EPL], span = 0.f;
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) total[j] = none;
-            for (int g = 0; g < a.n_groups; ++g) {
-                Best<V> b{none, 1 << 30};
+            for (int j = 0; j < EPL; ++j) v[j] = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-x[j])) : __expf(x[j] - at) * each;
+            if (a.bias)
 #pragma unroll
-                for (int j = 0; j < EPL; ++j)
-                    if (group[j] == g) better(b, v[j], j * LPR + t);
-                lane_best<LPR>(b);
-                V sum = b.v;
-                if (a.group_top > 1 && b.v > none) {
-                    Best<V> c{none, 1 << 30};
+                for (int j = 0; j < EPL; j += 4) {
+                    float b[4];
+                    load_part<float>(b, a.bias + e0 + j, a.n - e0 - j);
 #pragma unroll
-                    for (int j = 0; j < EPL; ++j)
-                        if (group[j] == g && j * LPR + t != b.e) better(c, v[j], j * LPR + t);
-                    lane_best<LPR>(c);
-                    if (c.v > none) sum += c.v;
+                    for (int i = 0; i < 4; ++i) {
+                        v[j + i] += b[i];
+                        if (fabsf(b[i]) < __builtin_huge_valf()) span = fmaxf(span, fabsf(b[i]));
+                    }
                 }
-#pragma unroll
-                for (int j = 0; j < EPL; ++j)
-                    if (j * LPR + t == g) total[j] = sum;
-            }
-            uint32_t keep = 0;
-            for (int q = 0; q < a.k_groups; ++q) {
-                Best<V> b{none, 1 << 30};
-#pragma unroll
-                for (int j = 0; j < EPL; ++j) better(b, total[j], j * LPR + t);
-                lane_best<LPR>(b);
-#pragma unroll
-                for (int j = 0; j < EPL; ++j) {
-                    if (b.v > none && group[j] == b.e) keep |= 1u << j;
-                    if (j * LPR + t == b.e) total[j] = none;
-                }
-            }
-            // without a bias the choice inside the groups goes by the logits (scores that saturate still differ there)
+            // In units of 2^-24: a row's scores are off by 4 (sigmoid) or by 43 of their own sum, which is at most 1 (softmax: 32 + 6
+            // additions, exp, the reciprocal), a sum with the bias by 1 + |bias| more; four values take part where two groups' two best
+            // are compared.  Decisions that hang on less than this are left to 64 bits.
+            const float margin = 6e-8f * (64.f + 8.f * lane_max<LPR>(span));
 #pragma unroll
             for (int j = 0; j < EPL; ++j) {
-                if (WIDE && !a.bias) v[j] = x[j];
-                if (!((keep >> j) & 1)) v[j] = none;
+                v[j] = x[j] > GATE_NONE ? v[j] : GATE_NONE;
+                bad = bad || v[j] != v[j];
+            }
+            if (a.n_groups > 1) gate_groups<LPR, EPL, LANES>(v, a, margin, near);
+            // without a bias the choice inside the groups goes by the logits (scores that saturate still differ there), read again: kept,
+            // they would cost every row 32 registers
+            if (!a.bias) {
+                float y[EPL];
+                gate_load<T, EPL>(y, a, row, r, e0, live);
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) v[j] = v[j] > GATE_NONE ? y[j] : GATE_NONE;
+            }
+            bad = group_ballot<LPR>(bad) != 0;
+            gate_choose<LPR, EPL>(v, a.k, a.bias != nullptr, margin, near, mine);
+            // rows whose choice hangs on fp32's error, one after the other, each by the whole wave
+            for (uint64_t doubt = __ballot(near && live && !bad && t == 0); doubt; doubt &= doubt - 1) {
+                const int own = ((int)(threadIdx.x & ~63) + __ffsll((unsigned long long)doubt) - 1) / LPR;
+                gate_exact<T, (LPR * EPL + 63) / 64>(a, r0 + own, chosen[own]);
             }
         }
-        int cell[KPL];
-#pragma unroll
-        for (int q = 0; q < KPL; ++q) cell[q] = -1;
-        for (int s = 0; s < a.k; ++s) {
-            Best<V> b{none, 1 << 30};
-#pragma unroll
-            for (int j = 0; j < EPL; ++j) better(b, v[j], j * LPR + t);
-            lane_best<LPR>(b);
-#pragma unroll
-            for (int j = 0; j < EPL; ++j)
-                if (j * LPR + t == b.e) v[j] = none;
-#pragma unroll
-            for (int q = 0; q < KPL; ++q)
-                if (q * LPR + t == s && b.v > none) cell[q] = b.e;
+        wave_sync();
+        // weights from the logits of the chosen: the largest of them, then the sum, then the weights (a lane's slots are few)
+        const int slots = live && !bad ? a.k : 0;
+        float base = GATE_NONE, total = 0.f;
+        auto log_score = [&](int c) {
+            const float l = (float)row[c];
+            return a.sigmoid ? log_sigmoid(l) : l;
+        };
+        if (a.renormalise) {
+            for (int s = t; s < slots; s += LPR)
+                if (mine[s] >= 0) base = fmaxf(base, log_score(mine[s]));
+            base = lane_max<LPR>(base);
+            if (!(base > GATE_NONE)) base = 0.f;
+            for (int s = t; s < slots; s += LPR)
+                if (mine[s] >= 0) total += expf(log_score(mine[s]) - base);
+            total = lane_sum<LPR>(total);
+        } else {
+            base = a.sigmoid ? 0.f : at;
+            total = all;
         }
-        // weights from the logits of the chosen
-        float w[KPL], total = 0.f, base = GATE_NONE;
-#pragma unroll
-        for (int q = 0; q < KPL; ++q) {
-            if (bad > 0.f) cell[q] = -1;
-            w[q] = cell[q] >= 0 ? (float)row[cell[q]] : GATE_NONE;
-            if (a.sigmoid && cell[q] >= 0) w[q] = log_sigmoid(w[q]);
-            base = fmaxf(base, w[q]);
-        }
-        if (a.renormalise) base = lane_max<LPR>(base);
-        else base = a.sigmoid ? 0.f : at;
-        if (!(base > GATE_NONE)) base = 0.f;
-#pragma unroll
-        for (int q = 0; q < KPL; ++q) {
-            w[q] = cell[q] >= 0 ? expf(w[q] - base) : 0.f;
-            total += w[q];
-        }
-        if (!a.renormalise) {
-            total = 0.f;
-#pragma unroll
-            for (int j = 0; j < EPL; ++j) total += x[j] > GATE_NONE ? expf(x[j] - at) : 0.f;
-        }
-        total = lane_sum<LPR>(total);
-        if (!a.renormalise && a.sigmoid) total = 1.f;
         if (!(total > 0.f)) total = 1.f;
         if (!live) continue;
-#pragma unroll
-        for (int q = 0; q < KPL; ++q) {
-            const int s = q * LPR + t;
-            if (s < a.k) {
-                cells[r * a.k + s] = cell[q];
-                weights[r * a.k + s] = bad > 0.f ? __builtin_nanf("") : w[q] / total * a.scale;
-            }
+        for (int s = t; s < a.k; s += LPR) {
+            const int c = bad ? -1 : mine[s];
+            cells[r * a.k + s] = c;
+            weights[r * a.k + s] = bad ? __builtin_nanf("") : c >= 0 ? expf(log_score(c) - base) / total * a.scale : 0.f;
         }
     }
 }
@@ -246,91 +433,89 @@ __global__ __launch_bounds__(256) void k_gate_fwd(float *__restrict__ weights, i
 template <class T, int LPR, int EPL>
 __global__ __launch_bounds__(256) void k_gate_bwd(T *__restrict__ dx, int64_t ldd, const float *__restrict__ dw, int64_t lddw,
                                                   const int32_t *__restrict__ cells, GateArgs a) {
-    constexpr int RPB = 256 / LPR, KPL = (GATE_MAX_K + LPR - 1) / LPR < EPL ? (GATE_MAX_K + LPR - 1) / LPR : EPL;
-    __shared__ float out[RPB][LPR * EPL];             // g of the chosen cells, 0 elsewhere
-    const int t = threadIdx.x % LPR, own = threadIdx.x / LPR;
+    constexpr int RPB = 256 / LPR;
+    __shared__ float out[RPB][LPR * EPL + 1];             // d of the chosen cells, 0 elsewhere; a group's own lanes alone use its row
+    const int t = threadIdx.x % LPR, e0 = t * EPL;
+    float *const mine = out[threadIdx.x / LPR];
+    const bool all = !a.sigmoid && !a.renormalise;        // the softmax over all open cells: all logits are read
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t r = r0 + own;
+        const int64_t r = r0 + threadIdx.x / LPR;
         const bool live = r < a.rows;
         const T *row = reinterpret_cast<const T *>(a.logits) + r * a.ldl;
-        int cell[KPL];
-        float x[KPL], g[KPL], base = GATE_NONE;
+        const int slots = live ? a.k : 0;
+        auto cell_of = [&](int s) {
+            const int c = cells[r * a.k + s];
+            return c < a.n ? c : -1;
+        };
+        auto log_score = [&](float l) { return a.sigmoid ? log_sigmoid(l) : l; };
+        wave_sync();                                      // the last row has been read
 #pragma unroll
-        for (int q = 0; q < KPL; ++q) {
-            const int s = q * LPR + t;
-            cell[q] = live && s < a.k ? cells[r * a.k + s] : -1;
-            if (cell[q] >= a.n) cell[q] = -1;
-            x[q] = cell[q] >= 0 ? (float)row[cell[q]] : GATE_NONE;
-            g[q] = cell[q] >= 0 ? dw[r * lddw + s] * a.scale : 0.f;
-        }
-        const bool all = !a.sigmoid && !a.renormalise;    // the softmax over all open cells: their logits are read again
-        float xa[EPL], total = 0.f;
+        for (int j = 0; j < EPL; ++j) mine[e0 + j] = 0.f;
+        // what the scores are relative to, their sum, and sum p g
+        float base = GATE_NONE, total = 0.f, mean = 0.f, some = -1.f, xa[EPL];
         if (all) {
+            gate_load<T, EPL>(xa, a, row, r, e0, live);
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) {
-                const int e = j * LPR + t;
-                bool open = live && e < a.n;
-                if (open && a.mask) open = a.mask[r * a.ldm + e] != 0;
-                xa[j] = open ? (float)row[e] : GATE_NONE;
-                base = fmaxf(base, xa[j]);
-            }
+            for (int j = 0; j < EPL; ++j) base = fmaxf(base, xa[j]);
         }
-        float some = -1.f;                                // a row without cells has no gradient
-#pragma unroll
-        for (int q = 0; q < KPL; ++q) some = fmaxf(some, (float)cell[q]);
+        for (int s = t; s < slots; s += LPR) {
+            const int c = cell_of(s);
+            some = fmaxf(some, (float)c);
+            if (c >= 0 && !all) base = fmaxf(base, log_score((float)row[c]));
+        }
         some = lane_max<LPR>(some);
-        float l[KPL];                                     // log of the score, up to a constant of the row
-#pragma unroll
-        for (int q = 0; q < KPL; ++q) {
-            l[q] = a.sigmoid && cell[q] >= 0 ? log_sigmoid(x[q]) : x[q];
-            if (!all) base = fmaxf(base, l[q]);
-        }
         base = lane_max<LPR>(base);
         if (!(base > GATE_NONE) || (a.sigmoid && !a.renormalise)) base = 0.f;
         if (all) {
 #pragma unroll
             for (int j = 0; j < EPL; ++j) {
-                xa[j] = xa[j] > GATE_NONE ? expf(xa[j] - base) : 0.f;
+                xa[j] = expf(xa[j] - base);
                 total += xa[j];
             }
         }
-        float p[KPL];
-#pragma unroll
-        for (int q = 0; q < KPL; ++q) {
-            p[q] = cell[q] >= 0 ? expf(l[q] - base) : 0.f;
-            if (!all) total += p[q];
+        for (int s = t; s < slots; s += LPR) {
+            const int c = cell_of(s);
+            if (c < 0) continue;
+            const float p = expf(log_score((float)row[c]) - base);
+            if (!all) total += p;
+            mean += p * (dw[r * lddw + s] * a.scale);
         }
         total = lane_sum<LPR>(total);
-        if (a.sigmoid && !a.renormalise) total = 1.f;
-        if (!(total > 0.f)) total = 1.f;
-        float mean = 0.f;
-#pragma unroll
-        for (int q = 0; q < KPL; ++q) {
-            p[q] /= total;
-            mean += p[q] * g[q];
-        }
         mean = lane_sum<LPR>(mean);
-        if (a.sigmoid && !a.renormalise) mean = 0.f;
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) out[own][j * LPR + t] = 0.f;
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < KPL; ++q) {
-            if (cell[q] < 0) continue;
-            float d = p[q] * (all ? g[q] : g[q] - mean);
-            if (a.sigmoid) d *= 1.f / (1.f + expf(x[q]));     // 1 - s
-            out[own][cell[q]] = d;
+        if (a.sigmoid && !a.renormalise) { total = 1.f; mean = 0.f; }
+        if (!(total > 0.f)) total = 1.f;
+        mean /= total;
+        wave_sync();                                      // the zeros are there
+        for (int s = t; s < slots; s += LPR) {
+            const int c = cell_of(s);
+            if (c < 0) continue;
+            const float l = (float)row[c], g = dw[r * lddw + s] * a.scale;
+            float d = expf(log_score(l) - base) / total * (all ? g : g - mean);
+            if (a.sigmoid) d *= 1.f / (1.f + expf(l));    // 1 - s
+            mine[c] = d;
         }
-        __syncthreads();
-        if (live)
+        wave_sync();
+        if (!live) continue;
+        constexpr int N = EPL < Vec<T>::N ? EPL : Vec<T>::N;
+        typedef T part __attribute__((ext_vector_type(N)));
+        typedef part part_at __attribute__((aligned(sizeof(T))));
+        T *to = dx + r * ldd + e0;
+        const float share = mean / total;
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) {
-                const int e = j * LPR + t;
-                float d = out[own][e];
-                if (all) d -= xa[j] / total * mean;
-                if (e < a.n) dx[r * ldd + e] = (T)(some >= 0.f ? d : 0.f);
+        for (int j = 0; j < EPL; j += N) {
+            part v;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float d = mine[e0 + j + i];
+                if (all) d -= xa[j + i] * share;
+                v[i] = (T)(some >= 0.f ? d : 0.f);        // (a row without cells has no gradient)
             }
-        __syncthreads();
+            if (e0 + j + N <= a.n) *reinterpret_cast<part_at *>(to + j) = v;
+            else
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (e0 + j + i < a.n) to[j + i] = v[i];
+        }
     }
 }
 
@@ -339,17 +524,17 @@ __global__ void k_gate_no_offsets(int32_t *__restrict__ offsets, int n) {
     if (c < n) offsets[c] = 0;
 }
 
-// lanes and cells per lane for n cells: the fewest lanes at up to 8 (above 512 cells 16) values each
+// lanes and cells per lane for n cells: the fewest lanes at up to 32 values each
 template <class F> static int gate_shape(int n, F &&f) {
     using std::integral_constant;
-    if (n <= 8) return f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-    if (n <= 16) return f(integral_constant<int, 8>{}, integral_constant<int, 2>{});
-    if (n <= 32) return f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
-    if (n <= 64) return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
-    if (n <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-    if (n <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    if (n <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
-    return f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    if (n <= 8) return f(integral_constant<int, 1>{}, integral_constant<int, 8>{});
+    if (n <= 16) return f(integral_constant<int, 1>{}, integral_constant<int, 16>{});
+    if (n <= 32) return f(integral_constant<int, 1>{}, integral_constant<int, 32>{});
+    if (n <= 64) return f(integral_constant<int, 2>{}, integral_constant<int, 32>{});
+    if (n <= 128) return f(integral_constant<int, 4>{}, integral_constant<int, 32>{});
+    if (n <= 256) return f(integral_constant<int, 8>{}, integral_constant<int, 32>{});
+    if (n <= 512) return f(integral_constant<int, 16>{}, integral_constant<int, 32>{});
+    return f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
 }
 
 static unsigned gate_blocks(int64_t rows, int rpb) {
@@ -358,11 +543,16 @@ static unsigned gate_blocks(int64_t rows, int rpb) {
 }
 
 template <class T> static int gate_forward(float *weights, int32_t *cells, const GateArgs &a, hipStream_t st) {
-    const bool wide = a.bias || (a.n_groups > 1 && a.group_top > 1);
+    const bool scored = a.bias || (a.n_groups > 1 && a.group_top > 1);
     return gate_shape(a.n, [&](auto lpr, auto epl) {
         constexpr int L = lpr, E = epl;
-        if (wide) hipLaunchKernelGGL((k_gate_fwd<T, L, E, double>), dim3(gate_blocks(a.rows, 256 / L)), dim3(256), 0, st, weights, cells, a);
-        else hipLaunchKernelGGL((k_gate_fwd<T, L, E, float>), dim3(gate_blocks(a.rows, 256 / L)), dim3(256), 0, st, weights, cells, a);
+        const int per_group = a.n / a.n_groups, lanes = per_group / E;
+        const bool whole = L > 1 && a.n_groups > 1 && per_group % E == 0 && (lanes & (lanes - 1)) == 0 && lanes < L;     // groups of whole lanes
+        const dim3 grid(gate_blocks(a.rows, 256 / L));
+        if (scored && whole) hipLaunchKernelGGL((k_gate_fwd<T, L, E, true, (L > 1)>), grid, dim3(256), 0, st, weights, cells, a);
+        else if (scored) hipLaunchKernelGGL((k_gate_fwd<T, L, E, true, false>), grid, dim3(256), 0, st, weights, cells, a);
+        else if (whole) hipLaunchKernelGGL((k_gate_fwd<T, L, E, false, (L > 1)>), grid, dim3(256), 0, st, weights, cells, a);
+        else hipLaunchKernelGGL((k_gate_fwd<T, L, E, false, false>), grid, dim3(256), 0, st, weights, cells, a);
         return check_launch("k_gate_fwd");
     });
 }

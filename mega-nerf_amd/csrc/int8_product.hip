@@ -325,17 +325,85 @@ __global__ __launch_bounds__(64 * WR * WC) void k_product(ProductArgs p, int n_t
 template <class T, int WR, int WC, int RB, int CB> static int tiled(const ProductArgs &p, int cus_per, hipStream_t st) {
     using S = Tile<WR, WC, RB, CB>;
     const int64_t nt = (p.n + S::BN - 1) / S::BN, total = nt * ((p.m + S::BM - 1) / S::BM);
-    if (p.lda > (1 << 22) || p.ldb > (1 << 22)) return set_err(MNR_E_INVALID, "the pitches of mnr_int8_product are at most 2^22 bytes");
     if (total >= (1ll << 30)) return set_err(MNR_E_INVALID, "the output of mnr_int8_product is too large (%lld tiles)", (long long)total);
     const int64_t most = 256ll * cus_per;
     hipLaunchKernelGGL((k_product<T, WR, WC, RB, CB>), dim3((unsigned)(total < most ? total : most)), dim3(S::THREADS), 0, st, p, (int)nt, (int)total);
     return check_launch("k_product");
 }
 
+// ---- few tiles: K split over the waves ---------------------------------------------------------------------------------------------
+// A workgroup of four waves makes 16 columns x 16 MT rows; wave w takes the 64-byte steps w, w + 4, ... of K straight from memory as
+// fragments of v_mfma_i32_16x16x64_i8 (a lane: 16 bytes of one row), four steps in flight, and the waves' int32 sums meet in LDS.  What
+// bounds it is the weight's bytes and the way to them: one row through 2048 x 2048 takes 4 MB and no reuse, 14.6 us by 16 tiles of 128 x
+// 128 and THIN_US by 128 of these workgroups.
+template <class T, int MT>
+__global__ __launch_bounds__(256) void k_product_thin(ProductArgs p) {
+    __shared__ int4v part[3][MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, quarter = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16 * MT;
+    const int k16 = (int)((p.k + 15) / 16 * 16), steps = (k16 + 63) / 64;
+    const int64_t nr = n0 + i16 < p.n ? n0 + i16 : p.n - 1;
+    const int8_t *b = p.b + nr * p.ldb, *a[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) a[i] = p.a + (m0 + i * 16 + i16 < p.m ? m0 + i * 16 + i16 : p.m - 1) * p.lda;
+    int4v acc[MT] = {};
+    constexpr int AHEAD = 4;
+    for (int s0 = wave; s0 < steps; s0 += 4 * AHEAD) {
+        int4v bf[AHEAD], af[AHEAD][MT];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int at = (s0 + 4 * u) * 64 + quarter * 16;
+            const bool in = at < k16;                  // behind k: the first piece again, times zero
+            bf[u] = *reinterpret_cast<const int4v *>(b + (in ? at : 0));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                af[u][i] = *reinterpret_cast<const int4v *>(a[i] + (in ? at : 0));
+                af[u][i] = in ? af[u][i] : int4v{0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[u], af[u][i], acc[i], 0, 0, 0);
+    }
+    if (wave)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) part[wave - 1][i][lane] = acc[i];
+    __syncthreads();
+    if (wave) return;
+    // lane -> row m0 + 16 i + i16, registers -> columns n0 + 4 quarter ...
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int w = 0; w < 3; ++w) acc[i] += part[w][i][lane];
+        const int64_t m = m0 + i * 16 + i16;
+        if (m >= p.m) continue;
+        const float sa = p.sa[m];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t n = n0 + quarter * 4 + j;
+            if (n >= p.n) continue;
+            float y = (float)acc[i][j] * sa * p.sb[n] + (p.bias ? p.bias[n] : 0.f);
+            if (p.relu && y < 0.f) y = 0.f;
+            reinterpret_cast<T *>(p.y)[m * p.ldy + n] = (T)y;
+        }
+    }
+}
+
+template <class T, int MT> static int thin(const ProductArgs &p, hipStream_t st) {
+    hipLaunchKernelGGL((k_product_thin<T, MT>), dim3((unsigned)((p.n + 15) / 16), (unsigned)((p.m + 16 * MT - 1) / (16 * MT))), dim3(256), 0, st, p);
+    return check_launch("k_product_thin");
+}
+
 template <class T> static int product(const ProductArgs &p, hipStream_t st) {
-    const int64_t big = ((p.m + 255) / 256) * ((p.n + 255) / 256);
+    // 256 x 256 tiles where they fill most of the chip, 128 x 128 tiles (two workgroups a CU) where those fill a fair part of it, and K
+    // split over waves below that
+    const int64_t big = ((p.m + 255) / 256) * ((p.n + 255) / 256), mid = ((p.m + 127) / 128) * ((p.n + 127) / 128);
     if (big >= 192) return tiled<T, 2, 4, 4, 2>(p, 1, st);
-    return tiled<T, 2, 2, 2, 2>(p, 2, st);
+    if (mid >= 96) return tiled<T, 2, 2, 2, 2>(p, 2, st);
+    if (p.m <= 16) return thin<T, 1>(p, st);
+    if (p.m <= 32) return thin<T, 2>(p, st);
+    return thin<T, 4>(p, st);
 }
 
 template <class T>
@@ -375,30 +443,55 @@ extern "C" int mnr_quantize_rows(int8_t *values_dev, int64_t pitch, float *scale
     return quantize<bf16_t>(values_dev, pitch, scale_dev, x_dev, ldx, rows, cols, st);
 }
 
-extern "C" size_t mnr_int8_product_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    (void)m; (void)n; (void)k;
-    return 0;
+static int product_check(const char *who, const void *y, int64_t ldy, const int8_t *b, int64_t ldb, const float *sb, int64_t m, int64_t n, int64_t k,
+                         int act, int type) {
+    MNR_REQUIRE(type_ok(type), "unknown element type passed to %s", who);
+    MNR_REQUIRE(act == 0 || act == 1, "the activation of %s is 0 (none) or 1 (ReLU)", who);
+    MNR_REQUIRE(m >= 0 && n >= 0 && m < (1ll << 31) && n < (1ll << 31), "%s needs 0 <= m, n < 2^31", who);
+    MNR_REQUIRE(k >= 1 && k <= 131071, "%s needs 1 <= k <= 131071: longer sums may leave int32", who);
+    if (m == 0 || n == 0) return MNR_OK;
+    const int64_t k16 = (k + 15) / 16 * 16;
+    MNR_REQUIRE(y && b && sb, "null pointer passed to %s", who);
+    MNR_REQUIRE((reinterpret_cast<uintptr_t>(b) & 15) == 0 && ldb % 16 == 0 && ldb < (1 << 22),
+                "the operands of %s start at multiples of 16 bytes, with pitches that are multiples of 16 below 2^22", who);
+    MNR_REQUIRE((n == 1 || ldb >= k16) && (m == 1 || ldy >= n), "row pitch smaller than a row passed to %s", who);
+    return MNR_OK;
 }
 
-extern "C" int mnr_int8_product(void *y_dev, int64_t ldy, const int8_t *a_dev, int64_t lda, const float *a_scale_dev, const int8_t *b_dev, int64_t ldb,
-                                const float *b_scale_dev, const float *bias_dev, int64_t m, int64_t n, int64_t k, int act, int type,
-                                void *workspace_dev, size_t workspace_bytes, void *stream) {
-    MNR_REQUIRE(type_ok(type), "unknown element type passed to mnr_int8_product");
-    MNR_REQUIRE(act == 0 || act == 1, "the activation of mnr_int8_product is 0 (none) or 1 (ReLU)");
-    MNR_REQUIRE(m >= 0 && n >= 0 && m < (1ll << 31) && n < (1ll << 31), "mnr_int8_product needs 0 <= m, n < 2^31");
-    MNR_REQUIRE(k >= 1 && k <= 131071, "mnr_int8_product needs 1 <= k <= 131071: longer sums may leave int32");
-    if (m == 0 || n == 0) return MNR_OK;
-    MNR_REQUIRE(y_dev && a_dev && a_scale_dev && b_dev && b_scale_dev, "null pointer passed to mnr_int8_product");
-    const int64_t k16 = (k + 15) / 16 * 16;
-    MNR_REQUIRE(((reinterpret_cast<uintptr_t>(a_dev) | reinterpret_cast<uintptr_t>(b_dev)) & 15) == 0 && lda % 16 == 0 && ldb % 16 == 0,
-                "a and b of mnr_int8_product start at multiples of 16 bytes, with pitches that are multiples of 16");
-    MNR_REQUIRE((m == 1 || lda >= k16) && (n == 1 || ldb >= k16) && (m == 1 || ldy >= n), "row pitch smaller than a row passed to mnr_int8_product");
-    MNR_REQUIRE(workspace_bytes >= mnr_int8_product_workspace_bytes(m, n, k), "mnr_int8_product needs %zu bytes of workspace",
-                mnr_int8_product_workspace_bytes(m, n, k));
-    (void)workspace_dev;
-    const ProductArgs p{y_dev, ldy, a_dev, lda, a_scale_dev, b_dev, ldb, b_scale_dev, bias_dev, m, n, k, act};
-    hipStream_t st = as_stream(stream);
+static int run_product(const ProductArgs &p, int type, hipStream_t st) {
     if (type == MNR_F32) return product<float>(p, st);
     if (type == MNR_F16) return product<f16_t>(p, st);
     return product<bf16_t>(p, st);
+}
+
+extern "C" int mnr_int8_product(void *y_dev, int64_t ldy, const int8_t *a_dev, int64_t lda, const float *a_scale_dev, const int8_t *b_dev, int64_t ldb,
+                                const float *b_scale_dev, const float *bias_dev, int64_t m, int64_t n, int64_t k, int act, int type, void *stream) {
+    const int rc = product_check("mnr_int8_product", y_dev, ldy, b_dev, ldb, b_scale_dev, m, n, k, act, type);
+    if (rc != MNR_OK || m == 0 || n == 0) return rc;
+    MNR_REQUIRE(a_dev && a_scale_dev, "null pointer passed to mnr_int8_product");
+    MNR_REQUIRE((reinterpret_cast<uintptr_t>(a_dev) & 15) == 0 && lda % 16 == 0 && lda < (1 << 22),
+                "the operands of mnr_int8_product start at multiples of 16 bytes, with pitches that are multiples of 16 below 2^22");
+    MNR_REQUIRE(m == 1 || lda >= (k + 15) / 16 * 16, "row pitch smaller than a row passed to mnr_int8_product");
+    return run_product(ProductArgs{y_dev, ldy, a_dev, lda, a_scale_dev, b_dev, ldb, b_scale_dev, bias_dev, m, n, k, act}, type, as_stream(stream));
+}
+
+static int64_t linear_pitch(int64_t k) { return (k + 127) / 128 * 128; }
+
+extern "C" size_t mnr_int8_linear_workspace_bytes(int64_t m, int64_t k) {
+    return m < 0 || k < 1 ? 0 : (size_t)m * (size_t)linear_pitch(k) + (size_t)m * sizeof(float);
+}
+
+extern "C" int mnr_int8_linear(void *y_dev, int64_t ldy, const void *x_dev, int64_t ldx, int x_type, const int8_t *b_dev, int64_t ldb,
+                               const float *b_scale_dev, const float *bias_dev, int64_t m, int64_t n, int64_t k, int act, int type,
+                               void *workspace_dev, size_t workspace_bytes, void *stream) {
+    int rc = product_check("mnr_int8_linear", y_dev, ldy, b_dev, ldb, b_scale_dev, m, n, k, act, type);
+    if (rc != MNR_OK || m == 0 || n == 0) return rc;
+    MNR_REQUIRE(workspace_dev && (reinterpret_cast<uintptr_t>(workspace_dev) & 15) == 0 && workspace_bytes >= mnr_int8_linear_workspace_bytes(m, k),
+                "mnr_int8_linear needs %zu bytes of workspace at a multiple of 16", mnr_int8_linear_workspace_bytes(m, k));
+    const int64_t pitch = linear_pitch(k);
+    int8_t *q = reinterpret_cast<int8_t *>(workspace_dev);
+    float *scale = reinterpret_cast<float *>(q + m * pitch);
+    rc = mnr_quantize_rows(q, pitch, scale, x_dev, ldx, m, k, x_type, stream);
+    if (rc != MNR_OK) return rc;
+    return run_product(ProductArgs{y_dev, ldy, q, pitch, scale, b_dev, ldb, b_scale_dev, bias_dev, m, n, k, act}, type, as_stream(stream));
 }

@@ -50,18 +50,29 @@ __global__ __launch_bounds__(256) void k_ln_fwd(T *__restrict__ y, int64_t ldy, 
 #pragma unroll
         for (int j = 0; j < (HOLD ? NCH : 1); ++j) ln_affine<V>(wv[j], bv[j], w, b, wtype, (j * TPR + t) * V, C - (j * TPR + t) * V);
     // (a group whose row is past the end runs along without loading or storing: lane and workgroup exchanges stay whole)
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    typename Vec<T>::raw ahead[NCH];                   // the next row's 16 bytes, on their way while this row is summed
+    auto fetch = [&](int64_t r) {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            const int c = (j * TPR + t) * V;
+            ahead[j] = load_raw<T>(x + r * ldx + c, r < rows ? C - c : 0);
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    fetch((int64_t)blockIdx.x * RPB + threadIdx.x / TPR);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += step) {
         const int64_t r = r0 + threadIdx.x / TPR;
         const bool live = r < rows;
         float v[NCH][V];
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            const int c = (j * TPR + t) * V;
-            load_part<T>(v[j], x + r * ldx + c, live ? C - c : 0);
+        for (int j = 0; j < NCH; ++j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) s += v[j][i];
-        }
+            for (int i = 0; i < V; ++i) {
+                v[j][i] = (float)ahead[j][i];
+                s += v[j][i];
+            }
+        fetch(r + step);
         // the mean of what is left after the first mean corrects its rounding: a row far from zero keeps its precision
         const float mean = row_sum<TPR>(s, lds) * inv;
         float q = 0.f, d = 0.f;
@@ -114,17 +125,30 @@ __global__ __launch_bounds__(256) void k_ln_bwd(T *__restrict__ dx, int64_t lddx
     for (int j = 0; j < NCH; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) sw[j][i] = sb[j][i] = 0.f;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    typename Vec<T>::raw xa[NCH], ga[NCH];             // the next row's, on their way while this row is summed
+    float mean_a, rstd_a;
+    auto fetch = [&](int64_t r) {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            const int c = (j * TPR + t) * V, n = r < rows ? C - c : 0;
+            xa[j] = load_raw<T>(x + r * ldx + c, n);
+            ga[j] = load_raw<T>(dy + r * lddy + c, n);
+        }
+        mean_a = r < rows ? mean_in[r] : 0.f;
+        rstd_a = r < rows ? rstd_in[r] : 0.f;
+    };
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    fetch((int64_t)blockIdx.x * RPB + threadIdx.x / TPR);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += step) {
         const int64_t r = r0 + threadIdx.x / TPR;
         const bool live = r < rows;
         float h[NCH][V], g[NCH][V];
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            const int c = (j * TPR + t) * V, n = live ? C - c : 0;
-            load_part<T>(h[j], x + r * ldx + c, n);
-            load_part<T>(g[j], dy + r * lddy + c, n);
-        }
-        const float mean = live ? mean_in[r] : 0.f, rstd = live ? rstd_in[r] : 0.f;
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) { h[j][i] = (float)xa[j][i]; g[j][i] = (float)ga[j][i]; }
+        const float mean = mean_a, rstd = rstd_a;
+        fetch(r + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
@@ -180,23 +204,31 @@ __global__ __launch_bounds__(256) void k_ln_bwd(T *__restrict__ dx, int64_t lddx
     }
 }
 
-// dw / db = sum of the workgroups' partial sums, in one fixed order: 32 columns x 32 phases per workgroup
+// dw / db = sum of the workgroups' partial sums, in one fixed order: 16 columns x 64 phases per workgroup
 __global__ __launch_bounds__(1024) void k_ln_join(void *__restrict__ dw, void *__restrict__ db, int wtype, const float *__restrict__ part,
                                                   int n_part, int C) {
-    __shared__ float lds[32][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), ph = threadIdx.x >> 5, which = blockIdx.y;
+    __shared__ float lds[64][17];
+    const int i = threadIdx.x & 15, c = blockIdx.x * 16 + i, ph = threadIdx.x >> 4, which = blockIdx.y;
     void *out = which ? db : dw;
     if (!out) return;
     float s = 0.f;
     if (c < C)
-        for (int p = ph; p < n_part; p += 32) s += part[((int64_t)p * 2 + which) * C + c];
-    lds[ph][threadIdx.x & 31] = s;
+#pragma unroll 4
+        for (int p = ph; p < n_part; p += 64) s += part[((int64_t)p * 2 + which) * C + c];
+    lds[ph][i] = s;
+    __syncthreads();
+    if (ph < 8) {
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += lds[ph * 8 + k][i];
+        lds[ph * 8][i] = s;                            // (read by this thread alone before)
+    }
     __syncthreads();
     if (ph == 0 && c < C) {
-        float a = 0.f;
+        s = 0.f;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) a += lds[k][threadIdx.x];
-        store_any(out, c, a, wtype);
+        for (int k = 0; k < 8; ++k) s += lds[k * 8][i];
+        store_any(out, c, s, wtype);
     }
 }
 
@@ -335,9 +367,9 @@ template <class F> static int ln_dispatch(LnShape s, F &&f) {
     return f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
 }
 
-// workgroups of the backward pass: each row group gets 8 rows or more to spread its 2 C partial sums over, at most 4 workgroups a CU
+// workgroups of the backward pass: each row group gets 4 rows or more to spread its 2 C partial sums over, at most 4 workgroups a CU
 static int64_t ln_bwd_blocks(int64_t rows, int tpr) {
-    const int64_t per = (256 / (tpr ? tpr : 256)) * 8, n = (rows + per - 1) / per;
+    const int64_t per = (256 / (tpr ? tpr : 256)) * 4, n = (rows + per - 1) / per;
     return n < 1 ? 1 : (n > 1024 ? 1024 : n);
 }
 static int64_t ln_strips(int64_t rows) { return rows < 64 ? 1 : (rows < 64 * 64 ? rows / 64 : 64); }
@@ -353,7 +385,7 @@ static int ln_forward(void *y, int64_t ldy, float *mean, float *rstd, const void
     }
     return ln_dispatch(s, [&](auto tpr, auto nch) {
         const int64_t n = (rows + 256 / tpr - 1) / (256 / tpr);
-        hipLaunchKernelGGL((k_ln_fwd<T, tpr, nch>), dim3((unsigned)(n < 4096 ? n : 4096)), dim3(256), 0, st, (T *)y, ldy, mean, rstd, (const T *)x, ldx,
+        hipLaunchKernelGGL((k_ln_fwd<T, tpr, nch>), dim3((unsigned)(n < 2048 ? n : 2048)), dim3(256), 0, st, (T *)y, ldy, mean, rstd, (const T *)x, ldx,
                            w, b, wtype, rows, (int)C, eps);
         return check_launch("k_ln_fwd");
     });
@@ -389,7 +421,7 @@ static int ln_backward(void *dx, int64_t lddx, void *dw, void *db, const void *d
         });
     }
     if (rc != MNR_OK || !sums) return rc;
-    hipLaunchKernelGGL(k_ln_join, dim3((unsigned)((C + 31) / 32), 2), dim3(1024), 0, st, dw, db, wtype, part, (int)n_part, (int)C);
+    hipLaunchKernelGGL(k_ln_join, dim3((unsigned)((C + 15) / 16), 2), dim3(1024), 0, st, dw, db, wtype, part, (int)n_part, (int)C);
     return check_launch("k_ln_join");
 }
 

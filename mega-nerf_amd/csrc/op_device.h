@@ -63,6 +63,16 @@ __device__ __forceinline__ void store_part(T *p, const float (&v)[Vec<T>::N], in
     }
 }
 
+// load_part's 16 bytes as they are: four registers until they are needed
+template <class T>
+__device__ __forceinline__ typename Vec<T>::raw load_raw(const T *p, int n) {
+    if (n >= Vec<T>::N) return *reinterpret_cast<const typename Vec<T>::type *>(p);
+    typename Vec<T>::raw x;
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) x[i] = i < n ? p[i] : (T)0.f;
+    return x;
+}
+
 // V elements of a vector of runtime type from element i on, of which the first n exist; the rest become 0
 template <int V>
 __device__ __forceinline__ void load_any_part(float (&v)[V], const void *p, int64_t i, int n, int type) {

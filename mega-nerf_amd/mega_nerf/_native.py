@@ -214,7 +214,7 @@ EXPORTS = [
     'mnr_mlp_backward_weights_multi_h2', 'mnr_mlp_forward_cells_h2', 'mnr_side_create', 'mnr_side_destroy', 'mnr_mlp_forward_cells_multi',
     'mnr_layer_norm_forward', 'mnr_layer_norm_backward_workspace_bytes', 'mnr_layer_norm_backward', 'mnr_embedding_forward',
     'mnr_embedding_backward_workspace_bytes', 'mnr_embedding_backward', 'mnr_gate_forward', 'mnr_gate_backward',
-    'mnr_gate_dispatch_workspace_bytes', 'mnr_gate_dispatch', 'mnr_quantize_rows', 'mnr_int8_product_workspace_bytes', 'mnr_int8_product',
+    'mnr_gate_dispatch_workspace_bytes', 'mnr_gate_dispatch', 'mnr_quantize_rows', 'mnr_int8_product', 'mnr_int8_linear_workspace_bytes', 'mnr_int8_linear',
     'mnr_calibrate', 'mnr_calibrate_scratch_bytes', 'mnr_calibrate_hog', 'mnr_render_route_workspace_bytes',
 ]
 
@@ -367,9 +367,10 @@ def lib() -> C.CDLL:
         _lib.mnr_gate_dispatch_workspace_bytes.argtypes = [i64, i32]
         _lib.mnr_gate_dispatch.argtypes = [p, p, p, i64, i32, p, size, p]
         _lib.mnr_quantize_rows.argtypes = [p, i64, p, p, i64, i64, i64, i32, p]
-        _lib.mnr_int8_product_workspace_bytes.restype = size
-        _lib.mnr_int8_product_workspace_bytes.argtypes = [i64, i64, i64]
-        _lib.mnr_int8_product.argtypes = [p, i64, p, i64, p, p, i64, p, p, i64, i64, i64, i32, i32, p, size, p]
+        _lib.mnr_int8_product.argtypes = [p, i64, p, i64, p, p, i64, p, p, i64, i64, i64, i32, i32, p]
+        _lib.mnr_int8_linear_workspace_bytes.restype = size
+        _lib.mnr_int8_linear_workspace_bytes.argtypes = [i64, i64]
+        _lib.mnr_int8_linear.argtypes = [p, i64, p, i64, i32, p, i64, p, p, i64, i64, i64, i32, i32, p, size, p]
         _lib.mnr_calibrate_scratch_bytes.restype = C.c_size_t
         _lib.mnr_calibrate.argtypes = [C.POINTER(Calibration), C.c_void_p, C.c_size_t, C.c_void_p]
         _lib.mnr_calibrate_hog.argtypes = [C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_void_p]

@@ -38,74 +38,78 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
 
 
 def _operand(q: QuantizedRows, name: str, zero_tail: bool):
-    """(tensor, rows, cols, pitch) of values that the kernel can read as they lie, else of a copy: 16-byte aligned rows, readable up to
-    the next multiple of 16 columns, and for the left operand zeros there (its tail cannot be known, so it is copied)."""
+    """(tensor, scale, rows, cols, pitch) of values that the kernel can read as they lie, else of a copy: 16-byte aligned rows, readable
+    up to the next multiple of 16 columns, and for the left operand zeros there (its tail cannot be known, so it is copied)."""
     v, s = q
     if v.dtype != torch.int8 or v.dim() != 2 or v.shape[1] == 0:
         raise N.NativeError('{}.values must be int8 [rows, cols] with a column at least (got {} {})'.format(name, v.dtype, tuple(v.shape)))
     if not v.is_cuda:
         N.require_device(v, name + '.values')
-    if s.dtype != torch.float32 or s.shape != v.shape[:1]:
-        raise N.NativeError('{}.scale must be float32 [{}] (got {} {})'.format(name, v.shape[0], s.dtype, tuple(s.shape)))
-    N.on_device_of(v, s, name + '.scale')
     rows, cols = v.shape
-    pitch, up = v.stride(0), (cols + 15) // 16 * 16
-    if rows <= 1:
-        pitch = max(pitch, up) // 16 * 16 if pitch % 16 else max(pitch, up)
-    ok = (v.stride(1) == 1 and pitch % 16 == 0 and pitch >= up and v.data_ptr() % 16 == 0 and not (zero_tail and up > cols) and
-          v.storage_offset() + max(rows - 1, 0) * pitch + up <= v.untyped_storage().nbytes())
-    if not ok:
+    if s.dtype != torch.float32 or s.dim() != 1 or s.shape[0] != rows:
+        raise N.NativeError('{}.scale must be float32 [{}] (got {} {})'.format(name, rows, s.dtype, tuple(s.shape)))
+    N.on_device_of(v, s, name + '.scale')
+    up = (cols + 15) // 16 * 16
+    pitch = v.stride(0) if rows > 1 else up
+    if not (v.stride(1) == 1 and pitch % 16 == 0 and pitch >= up and pitch < 1 << 22 and v.data_ptr() % 16 == 0 and not (zero_tail and up > cols) and
+            v.storage_offset() + max(rows - 1, 0) * pitch + up <= v.untyped_storage().nbytes()):
         pitch = (cols + _PITCH - 1) // _PITCH * _PITCH
-        held = torch.zeros(rows, pitch, dtype=torch.int8, device=v.device)
+        held = v.new_zeros((rows, pitch))
         held[:, :cols] = v
         v = held
-    return v, rows, cols, pitch
+    return v, s.contiguous(), rows, cols, pitch
 
 
-def _product(a, m, k, lda, a_scale, b: QuantizedRows, bias, relu, out_dtype) -> torch.Tensor:
-    bv, n, kb, ldb = _operand(b, 'weight', False)
-    N.on_device_of(a, bv, 'weight')
-    if kb != k:
-        raise N.NativeError('the input has {} columns, the weight {}'.format(k, kb))
+def _epilogue(x: torch.Tensor, n: int, bias: Optional[torch.Tensor], out_dtype: torch.dtype):
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.shape != (n,):
+        if bias.dtype != torch.float32 or bias.dim() != 1 or bias.shape[0] != n:
             raise N.NativeError('bias must be float32 [{}] (got {} {})'.format(n, bias.dtype, tuple(bias.shape)))
-        N.on_device_of(a, bias, 'bias')
+        N.on_device_of(x, bias, 'bias')
         bias = bias.contiguous()
     code = N.ELEMENT_TYPES.get(out_dtype)
     if code is None:
         raise N.NativeError('the output is float32, float16 or bfloat16 (got {})'.format(out_dtype))
-    a_scale, b_scale = a_scale.contiguous(), b.scale.contiguous()
-    y = a.new_empty((m, n), dtype=out_dtype)
-    lib = N.lib()
-    size = lib.mnr_int8_product_workspace_bytes(m, n, k)
-    ws = a.new_empty(size, dtype=torch.uint8) if size else None
-    N.launch(a, lib.mnr_int8_product, y.data_ptr(), n, a.data_ptr(), lda, a_scale.data_ptr(), bv.data_ptr(), ldb, b_scale.data_ptr(),
-             N.ptr(bias), m, n, k, 1 if relu else 0, code, N.ptr(ws), size)
-    return y
+    return bias, code
 
 
 def int8_product(a: QuantizedRows, b: QuantizedRows, bias: Optional[torch.Tensor] = None, relu: bool = False,
                  out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """[M, N] = a [M, K] times the transpose of b [N, K] (+ bias float32 [N], ReLU): the integer sums are exact (K <= 131071), scaled in
     fp32 and rounded once to ``out_dtype``."""
-    av, m, k, lda = _operand(a, 'a', True)
-    return _product(av, m, k, lda, a.scale, b, bias, relu, out_dtype)
+    av, sa, m, k, lda = _operand(a, 'a', True)
+    bv, sb, n, kb, ldb = _operand(b, 'weight', False)
+    N.on_device_of(av, bv, 'weight')
+    if kb != k:
+        raise N.NativeError('the input has {} columns, the weight {}'.format(k, kb))
+    bias, code = _epilogue(av, n, bias, out_dtype)
+    y = av.new_empty((m, n), dtype=out_dtype)
+    N.launch(av, N.lib().mnr_int8_product, y.data_ptr(), n, av.data_ptr(), lda, sa.data_ptr(), bv.data_ptr(), ldb, sb.data_ptr(), N.ptr(bias), m, n, k,
+             1 if relu else 0, code)
+    return y
 
 
 def int8_linear(x: torch.Tensor, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, relu: bool = False,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """A dense layer served in 8 bits: x [..., K] is quantised row by row, multiplied with ``weight`` = ``quantize_rows(w)`` of an
-    nn.Linear weight [N, K], scaled, ``bias`` added, ReLU if ``relu``; [..., N] of x's type, or ``out_dtype``."""
+    """A dense layer served in 8 bits: x [..., K] is quantised row by row (as :func:`quantize_rows`), multiplied with ``weight`` =
+    ``quantize_rows(w)`` of an nn.Linear weight [N, K], scaled, ``bias`` added, ReLU if ``relu``; [..., N] of x's type, or
+    ``out_dtype``."""
     if x.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError('int8_linear is inference-only (use torch.no_grad())')
-    N.element_type(x, 'x')
+    xcode = N.element_type(x, 'x')
     shape = x.shape
-    if x.dim() != 2:
-        if x.dim() == 0 or shape[-1] == 0:
-            raise N.NativeError('int8_linear expects [..., K] with a column at least (got {})'.format(tuple(shape)))
-        x = x.reshape(-1, shape[-1])
-    q = quantize_rows(x)
-    m, k = q.values.shape
-    y = _product(q.values, m, k, (k + _PITCH - 1) // _PITCH * _PITCH, q.scale, weight, bias, relu, x.dtype if out_dtype is None else out_dtype)
-    return y if len(shape) == 2 else y.view(*shape[:-1], y.shape[1])
+    if x.dim() == 0 or shape[-1] == 0:
+        raise N.NativeError('int8_linear expects [..., K] with a column at least (got {})'.format(tuple(shape)))
+    x, m, k, ldx = N.matrix(x)
+    bv, sb, n, kb, ldb = _operand(weight, 'weight', False)
+    N.on_device_of(x, bv, 'weight')
+    if kb != k:
+        raise N.NativeError('the input has {} columns, the weight {}'.format(k, kb))
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    bias, code = _epilogue(x, n, bias, out_dtype)
+    y = x.new_empty(shape[:-1] + (n,), dtype=out_dtype)
+    lib = N.lib()
+    size = lib.mnr_int8_linear_workspace_bytes(m, k)
+    ws = x.new_empty(size, dtype=torch.uint8)
+    N.launch(x, lib.mnr_int8_linear, y.data_ptr(), n, x.data_ptr(), ldx, xcode, bv.data_ptr(), ldb, sb.data_ptr(), N.ptr(bias), m, n, k, 1 if relu else 0,
+             code, ws.data_ptr(), size)
+    return y

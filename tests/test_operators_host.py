@@ -148,9 +148,9 @@ def test_product_entry_refusals():
     refused(quant(ld=99), 'pitch')
     refused(quant(t=9), 'element type')
     assert quant(rows=0) == 0
-    names = ('y', 'ldy', 'a', 'lda', 'sa', 'b', 'ldb', 'sb', 'bias', 'm', 'n', 'k', 'act', 't', 'ws', 'size', 'st')
-    base = dict(y=P, ldy=32, a=P, lda=128, sa=P, b=P, ldb=128, sb=P, bias=None, m=4, n=32, k=100, act=0, t=0, ws=None, size=0, st=None)
-    prod = lambda **k: lib.mnr_int8_product(*[{**base, 'size': lib.mnr_int8_product_workspace_bytes(4, 32, 100), 'ws': P, **k}[a] for a in names])      # noqa: E731
+    names = ('y', 'ldy', 'a', 'lda', 'sa', 'b', 'ldb', 'sb', 'bias', 'm', 'n', 'k', 'act', 't', 'st')
+    base = dict(y=P, ldy=32, a=P, lda=128, sa=P, b=P, ldb=128, sb=P, bias=None, m=4, n=32, k=100, act=0, t=0, st=None)
+    prod = lambda **k: lib.mnr_int8_product(*[{**base, **k}[a] for a in names])      # noqa: E731
     refused(prod(k=0), 'k <=')
     refused(prod(k=131072, lda=131072, ldb=131072), 'k <=')
     refused(prod(a=P + 4), 'multiples of 16')
@@ -161,7 +161,19 @@ def test_product_entry_refusals():
     refused(prod(act=2), 'activation')
     refused(prod(b=None), 'null')
     refused(prod(m=-1), 'm, n')
+    refused(prod(lda=1 << 22), 'below 2^22')
     assert prod(m=0) == 0 and prod(n=0) == 0
+    need = lib.mnr_int8_linear_workspace_bytes(4, 100)
+    assert need == 4 * 128 + 16
+    linear = lambda **k: lib.mnr_int8_linear(*[{**base, 'x': P, 'ldx': 100, 'xt': 0, 'ws': P, 'size': need, **k}[a] for a in (      # noqa: E731
+        'y', 'ldy', 'x', 'ldx', 'xt', 'b', 'ldb', 'sb', 'bias', 'm', 'n', 'k', 'act', 't', 'ws', 'size', 'st')])
+    refused(linear(size=need - 1), 'workspace')
+    refused(linear(ws=P + 8), 'workspace')
+    refused(linear(xt=3), 'element type')
+    refused(linear(t=3), 'element type')
+    refused(linear(ldx=99), 'pitch')
+    refused(linear(k=131072), 'k <=')
+    assert linear(m=0) == 0
 
 
 def test_every_argument_list_matches_the_header():
@@ -172,7 +184,7 @@ def test_every_argument_list_matches_the_header():
     lib = N.lib()
     for name in ('mnr_layer_norm_forward', 'mnr_layer_norm_backward', 'mnr_layer_norm_backward_workspace_bytes', 'mnr_embedding_forward', 'mnr_embedding_backward',
                  'mnr_embedding_backward_workspace_bytes', 'mnr_gate_forward', 'mnr_gate_backward', 'mnr_gate_dispatch', 'mnr_gate_dispatch_workspace_bytes',
-                 'mnr_quantize_rows', 'mnr_int8_product', 'mnr_int8_product_workspace_bytes'):
+                 'mnr_quantize_rows', 'mnr_int8_product', 'mnr_int8_linear', 'mnr_int8_linear_workspace_bytes'):
         args = re.search(r'\b%s\(([^;]*)\);' % name, hdr).group(1).split(',')
         want = [C.c_void_p if '*' in a else C.c_int64 if 'int64_t' in a else C.c_size_t if 'size_t' in a else C.c_float if 'float' in a else C.c_int for a in args]
         assert list(getattr(lib, name).argtypes) == want, name
