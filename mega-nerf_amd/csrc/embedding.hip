@@ -184,13 +184,18 @@ __global__ __launch_bounds__(256) void k_emb_join(void *__restrict__ grad, int g
             const int o = longer[l], k = owner[o];
             const int64_t t = b0 + o;
             int64_t last = t + spans[o];
-            if (spans[o] == 0) {                       // first place behind the run
+            if (spans[o] == 0) {
+                // first place behind the run, in [lo, hi]: 256 probes at a time (each place before it holds k, none behind it)
                 int64_t lo = (t + 2) * EMB_TILE, hi = n;
                 while (lo < hi) {
-                    const int64_t mid = (lo + hi) >> 1;
-                    if (keys[mid] == k) lo = mid + 1; else hi = mid;
+                    const int64_t each = (hi - lo + 255) / 256, at = lo + each * threadIdx.x;
+                    const int64_t in = __syncthreads_count(at < hi && keys[at < hi ? at : lo] == k);         // probes inside the run
+                    if (in == 0) { hi = lo; break; }
+                    const int64_t from = lo + each * (in - 1) + 1, upto = lo + each * in;
+                    lo = from;
+                    hi = upto < hi ? upto : hi;
                 }
-                last = (lo - 1) / EMB_TILE;
+                last = (hi - 1) / EMB_TILE;
             }
             float acc[V];
 #pragma unroll

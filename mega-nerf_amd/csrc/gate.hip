@@ -47,6 +47,22 @@ template <int STEP> __device__ __forceinline__ void halves_of(double x, double &
     a = __longlong_as_double((long long)(((uint64_t)ph << 32) | pl));
     b = __longlong_as_double((long long)(((uint64_t)qh << 32) | ql));
 }
+// fp32 values are compared as whole numbers of the same order (one instruction for a maximum of three, and no care for NaNs; -0 counts as
+// 0).  none<V>() is what -inf becomes.
+__device__ __forceinline__ int key_of(float x) {
+    const int b = __float_as_int(x + 0.f);
+    return b ^ (b >> 31 & 0x7fffffff);
+}
+__device__ __forceinline__ float value_of(int k) { return __int_as_float(k ^ (k >> 31 & 0x7fffffff)); }
+__device__ __forceinline__ double value_of(double v) { return v; }
+__device__ __forceinline__ int max_of(int a, int b) { return max(a, b); }
+__device__ __forceinline__ int min_of(int a, int b) { return min(a, b); }
+__device__ __forceinline__ double max_of(double a, double b) { return b > a ? b : a; }
+__device__ __forceinline__ double min_of(double a, double b) { return b < a ? b : a; }
+template <class V> __device__ __forceinline__ V none_of();
+template <> __device__ __forceinline__ int none_of<int>() { return (int)0x807fffff; }
+template <> __device__ __forceinline__ double none_of<double>() { return -__builtin_huge_val(); }
+
 template <class V> __device__ __forceinline__ void better(Best<V> &a, V v, int e) {
     if (v > a.v || (v == a.v && e < a.e)) { a.v = v; a.e = e; }
 }
@@ -143,7 +159,24 @@ template <int LPR> __device__ __forceinline__ uint64_t group_ballot(bool b) {
     if constexpr (LPR == 64) return m;
     return (m >> ((threadIdx.x & 63) / LPR * LPR)) & ((1ull << LPR) - 1);
 }
-template <int LPR> __device__ __forceinline__ float group_max(float x) { return lane_max<LPR>(x); }
+template <int STEP> __device__ __forceinline__ int max_step(int x) {
+    if constexpr (STEP >= 16) {
+        int a, b;
+        halves_of<STEP>(x, a, b);
+        return max(a, b);
+    } else {
+        return max(x, other_of<STEP>(x));
+    }
+}
+template <int LPR> __device__ __forceinline__ int group_max(int x) {
+    if constexpr (LPR >= 2) x = max_step<1>(x);
+    if constexpr (LPR >= 4) x = max_step<2>(x);
+    if constexpr (LPR >= 8) x = max_step<4>(x);
+    if constexpr (LPR >= 16) x = max_step<8>(x);
+    if constexpr (LPR >= 32) x = max_step<16>(x);
+    if constexpr (LPR >= 64) x = max_step<32>(x);
+    return x;
+}
 template <int LPR> __device__ __forceinline__ double group_max(double x) {
     Best<double> b{x, 0};
     lane_best<LPR>(b);
@@ -152,10 +185,10 @@ template <int LPR> __device__ __forceinline__ double group_max(double x) {
 
 // Takes the largest of the group's values out of v: its value, and on the lane that had it `mine` = its number there, else -1
 template <int LPR, int EPL, class V> __device__ __forceinline__ V take_best(V (&v)[EPL], int &mine) {
-    const V none = (V)GATE_NONE;
+    const V none = none_of<V>();
     V high = v[0];
 #pragma unroll
-    for (int j = 1; j < EPL; ++j) high = v[j] > high ? v[j] : high;
+    for (int j = 1; j < EPL; ++j) high = max_of(high, v[j]);
     const V best = group_max<LPR>(high);
     bool own = best > none;
     if constexpr (LPR > 1) {
@@ -175,9 +208,14 @@ template <int LPR, int EPL, class V> __device__ __forceinline__ V take_best(V (&
 
 // The two largest of two pairs of (largest, second)
 template <class V> __device__ __forceinline__ void merge_two(V &a1, V &a2, V b1, V b2) {
-    const V low = a1 < b1 ? a1 : b1, high = a1 < b1 ? b1 : a1, second = a2 < b2 ? b2 : a2;
-    a1 = high;
-    a2 = low < second ? second : low;
+    const V low = min_of(a1, b1);
+    a1 = max_of(a1, b1);
+    a2 = max_of(low, max_of(a2, b2));
+}
+template <class V> __device__ __forceinline__ void merge_one(V &a1, V &a2, V b) {
+    const V low = min_of(a1, b);
+    a1 = max_of(a1, b);
+    a2 = max_of(a2, low);
 }
 template <int STEP, class V> __device__ __forceinline__ void merge_two_step(V &a1, V &a2) {
     if constexpr (STEP >= 16) {
@@ -198,32 +236,37 @@ template <int LANES, class V> __device__ __forceinline__ void merge_two_lanes(V 
     if constexpr (LANES >= 32) merge_two_step<16>(a1, a2);
     if constexpr (LANES >= 64) merge_two_step<32>(a1, a2);
 }
-template <class V> __device__ __forceinline__ V group_total(V a1, V a2, int top) {
-    return top > 1 && a2 > (V)GATE_NONE ? a1 + a2 : a1;      // (a1 none: none)
+__device__ __forceinline__ int group_total(int a1, int a2, int top) {
+    return top > 1 && a2 > none_of<int>() ? key_of(value_of(a1) + value_of(a2)) : a1;      // (a1 none: none)
 }
+__device__ __forceinline__ double group_total(double a1, double a2, int top) { return top > 1 && a2 > none_of<double>() ? a1 + a2 : a1; }
+// whether two values that a decision kept apart are closer than `margin`
+__device__ __forceinline__ bool too_near(int a, int b, float margin) { return b > none_of<int>() && value_of(a) - value_of(b) <= margin; }
+__device__ __forceinline__ bool too_near(double, double, float) { return false; }
 
 // Closes the cells of the groups that are not among the best k_groups.  `near` becomes true where the choice hangs on a difference of at
 // most `margin`.  LANES: a group is the cells of a power of two of whole lanes (one pass for all groups); else any size, group by group.
 template <int LPR, int EPL, bool LANES, class V>
-__device__ __forceinline__ void gate_groups(V (&v)[EPL], const GateArgs &a, V margin, bool &near) {
-    const V none = (V)GATE_NONE;
+__device__ __forceinline__ void gate_groups(V (&v)[EPL], const GateArgs &a, float margin, bool &near) {
+    const V none = none_of<V>();
     const int t = threadIdx.x % LPR, per_group = a.n / a.n_groups;
     V last = none;
     if constexpr (LANES) {
         const int lanes = per_group / EPL;
         V a1 = v[0], a2 = none;
 #pragma unroll
-        for (int j = 1; j < EPL; ++j) merge_two(a1, a2, v[j], none);
+        for (int j = 1; j < EPL; ++j) merge_one(a1, a2, v[j]);
         if constexpr (LPR >= 4) { if (lanes >= 2) merge_two_step<1>(a1, a2); }
         if constexpr (LPR >= 8) { if (lanes >= 4) merge_two_step<2>(a1, a2); }
         if constexpr (LPR >= 16) { if (lanes >= 8) merge_two_step<4>(a1, a2); }
         if constexpr (LPR >= 32) { if (lanes >= 16) merge_two_step<8>(a1, a2); }
+        if constexpr (LPR >= 64) { if (lanes >= 32) merge_two_step<16>(a1, a2); }
         V total[1] = {(t & (lanes - 1)) == 0 ? group_total(a1, a2, a.group_top) : none};         // its first lane holds it
         bool keep = false;
         for (int q = 0; q <= a.k_groups && q < a.n_groups; ++q) {
             int mine;
             const V best = take_best<LPR, 1>(total, mine);
-            if (q == a.k_groups) near = near || (best > none && last - best <= margin);
+            if (q == a.k_groups) near = near || too_near(last, best, margin);
             else {
                 last = best;
                 const uint64_t who = group_ballot<LPR>(mine >= 0);
@@ -241,7 +284,7 @@ __device__ __forceinline__ void gate_groups(V (&v)[EPL], const GateArgs &a, V ma
             // this lane's cells of group g: from `from` up to `from + per_group`
             const int from = g * per_group - t * EPL;
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) merge_two(a1, a2, (unsigned)(j - from) < (unsigned)per_group ? v[j] : none, none);
+            for (int j = 0; j < EPL; ++j) merge_one(a1, a2, (unsigned)(j - from) < (unsigned)per_group ? v[j] : none);
             merge_two_lanes<LPR>(a1, a2);
 #pragma unroll
             for (int j = 0; j < EPL; ++j)
@@ -251,7 +294,7 @@ __device__ __forceinline__ void gate_groups(V (&v)[EPL], const GateArgs &a, V ma
         for (int q = 0; q <= a.k_groups && q < a.n_groups; ++q) {
             int mine;
             const V best = take_best<LPR, EPL>(total, mine);
-            if (q == a.k_groups) near = near || (best > none && last - best <= margin);
+            if (q == a.k_groups) near = near || too_near(last, best, margin);
             else {
                 last = best;
                 int g = mine;                          // which group that was, for all lanes
@@ -274,19 +317,19 @@ __device__ __forceinline__ void gate_groups(V (&v)[EPL], const GateArgs &a, V ma
 // Writes the chosen cells to `chosen` [k] (LDS, -1 where there are no more).  `near` as above, over the order of the chosen and the last
 // one's lead over the rest.
 template <int LPR, int EPL, class V>
-__device__ __forceinline__ void gate_choose(V (&v)[EPL], int k, bool check, V margin, bool &near, int *chosen) {
+__device__ __forceinline__ void gate_choose(V (&v)[EPL], int k, bool check, float margin, bool &near, int *chosen) {
     const int t = threadIdx.x % LPR;
-    V last = (V)__builtin_huge_valf();
+    V last = none_of<V>();
     for (int s = 0; s < k + (check ? 1 : 0); ++s) {
         int mine;
         const V best = take_best<LPR, EPL>(v, mine);
         if (check) {                                   // (uniform)
-            near = near || (best > (V)GATE_NONE && s > 0 && last - best <= margin);
+            near = near || (s > 0 && too_near(last, best, margin));
             last = best;
         }
         if (s < k) {
             if (mine >= 0) chosen[s] = t * EPL + mine;
-            else if (t == 0 && !(best > (V)GATE_NONE)) chosen[s] = -1;
+            else if (t == 0 && !(best > none_of<V>())) chosen[s] = -1;
         }
     }
 }
@@ -313,11 +356,11 @@ template <class T, int EPL> __device__ __forceinline__ void gate_exact(const Gat
         v[j] = x[j] > GATE_NONE ? v[j] : (double)GATE_NONE;
     }
     bool done = false;
-    if (a.n_groups > 1) gate_groups<64, EPL, false>(v, a, -1., done);
+    if (a.n_groups > 1) gate_groups<64, EPL, false>(v, a, -1.f, done);
     if (!a.bias)
 #pragma unroll
         for (int j = 0; j < EPL; ++j) v[j] = v[j] > (double)GATE_NONE ? (double)x[j] : (double)GATE_NONE;
-    gate_choose<64, EPL>(v, a.k, false, -1., done, chosen);
+    gate_choose<64, EPL>(v, a.k, false, -1.f, done, chosen);
 }
 
 // LPR lanes share a row, lane t holds cells t EPL ... and slots t, t + LPR, ...
@@ -350,9 +393,9 @@ __global__ __launch_bounds__(256, SCORED ? 2 : 4) void k_gate_fwd(float *__restr
         }
         wave_sync();                                         // the last row's list has been read
         if constexpr (!SCORED) {
-            float v[EPL];
+            int v[EPL];
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) v[j] = x[j];
+            for (int j = 0; j < EPL; ++j) v[j] = key_of(x[j]);
             bool exact = false;
             if (a.n_groups > 1) gate_groups<LPR, EPL, LANES>(v, a, -1.f, exact);
             bad = group_ballot<LPR>(bad) != 0;
@@ -360,9 +403,9 @@ __global__ __launch_bounds__(256, SCORED ? 2 : 4) void k_gate_fwd(float *__restr
         } else {
             bool near = false;
             const float each = all > 0.f ? 1.f / all : 0.f;
-            float v[EPL], span = 0.f;
+            float w[EPL], span = 0.f;
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) v[j] = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-x[j])) : __expf(x[j] - at) * each;
+            for (int j = 0; j < EPL; ++j) w[j] = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-x[j])) : __expf(x[j] - at) * each;
             if (a.bias)
 #pragma unroll
                 for (int j = 0; j < EPL; j += 4) {
@@ -370,7 +413,7 @@ __global__ __launch_bounds__(256, SCORED ? 2 : 4) void k_gate_fwd(float *__restr
                     load_part<float>(b, a.bias + e0 + j, a.n - e0 - j);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        v[j + i] += b[i];
+                        w[j + i] += b[i];
                         if (fabsf(b[i]) < __builtin_huge_valf()) span = fmaxf(span, fabsf(b[i]));
                     }
                 }
@@ -378,10 +421,12 @@ __global__ __launch_bounds__(256, SCORED ? 2 : 4) void k_gate_fwd(float *__restr
             // additions, exp, the reciprocal), a sum with the bias by 1 + |bias| more; four values take part where two groups' two best
             // are compared.  Decisions that hang on less than this are left to 64 bits.
             const float margin = 6e-8f * (64.f + 8.f * lane_max<LPR>(span));
+            int v[EPL];
 #pragma unroll
             for (int j = 0; j < EPL; ++j) {
-                v[j] = x[j] > GATE_NONE ? v[j] : GATE_NONE;
-                bad = bad || v[j] != v[j];
+                const bool open = x[j] > GATE_NONE;
+                bad = bad || (open && w[j] != w[j]);
+                v[j] = open ? key_of(w[j]) : none_of<int>();
             }
             if (a.n_groups > 1) gate_groups<LPR, EPL, LANES>(v, a, margin, near);
             // without a bias the choice inside the groups goes by the logits (scores that saturate still differ there), read again: kept,
@@ -390,7 +435,7 @@ __global__ __launch_bounds__(256, SCORED ? 2 : 4) void k_gate_fwd(float *__restr
                 float y[EPL];
                 gate_load<T, EPL>(y, a, row, r, e0, live);
 #pragma unroll
-                for (int j = 0; j < EPL; ++j) v[j] = v[j] > GATE_NONE ? y[j] : GATE_NONE;
+                for (int j = 0; j < EPL; ++j) v[j] = v[j] > none_of<int>() ? key_of(y[j]) : none_of<int>();
             }
             bad = group_ballot<LPR>(bad) != 0;
             gate_choose<LPR, EPL>(v, a.k, a.bias != nullptr, margin, near, mine);
@@ -524,17 +569,19 @@ __global__ void k_gate_no_offsets(int32_t *__restrict__ offsets, int n) {
     if (c < n) offsets[c] = 0;
 }
 
-// lanes and cells per lane for n cells: the fewest lanes at up to 32 values each
-template <class F> static int gate_shape(int n, F &&f) {
+// lanes and cells per lane for n cells: the fewest lanes at up to MOST (32, or 16 where scores are compared: with 32 those kernels take
+// 220 registers, two waves a SIMD) values each
+template <int MOST, class F> static int gate_shape(int n, F &&f) {
     using std::integral_constant;
     if (n <= 8) return f(integral_constant<int, 1>{}, integral_constant<int, 8>{});
     if (n <= 16) return f(integral_constant<int, 1>{}, integral_constant<int, 16>{});
-    if (n <= 32) return f(integral_constant<int, 1>{}, integral_constant<int, 32>{});
-    if (n <= 64) return f(integral_constant<int, 2>{}, integral_constant<int, 32>{});
-    if (n <= 128) return f(integral_constant<int, 4>{}, integral_constant<int, 32>{});
-    if (n <= 256) return f(integral_constant<int, 8>{}, integral_constant<int, 32>{});
-    if (n <= 512) return f(integral_constant<int, 16>{}, integral_constant<int, 32>{});
-    return f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    if (n <= MOST) return f(integral_constant<int, 1>{}, integral_constant<int, MOST>{});
+    if (n <= 2 * MOST) return f(integral_constant<int, 2>{}, integral_constant<int, MOST>{});
+    if (n <= 4 * MOST) return f(integral_constant<int, 4>{}, integral_constant<int, MOST>{});
+    if (n <= 8 * MOST) return f(integral_constant<int, 8>{}, integral_constant<int, MOST>{});
+    if (n <= 16 * MOST) return f(integral_constant<int, 16>{}, integral_constant<int, MOST>{});
+    if (n <= 32 * MOST) return f(integral_constant<int, 32>{}, integral_constant<int, MOST>{});
+    return f(integral_constant<int, 64>{}, integral_constant<int, 1024 / 64>{});
 }
 
 static unsigned gate_blocks(int64_t rows, int rpb) {
@@ -542,23 +589,24 @@ static unsigned gate_blocks(int64_t rows, int rpb) {
     return (unsigned)(n < 8192 ? n : 8192);
 }
 
-template <class T> static int gate_forward(float *weights, int32_t *cells, const GateArgs &a, hipStream_t st) {
-    const bool scored = a.bias || (a.n_groups > 1 && a.group_top > 1);
-    return gate_shape(a.n, [&](auto lpr, auto epl) {
+template <class T, bool SCORED> static int gate_forward_as(float *weights, int32_t *cells, const GateArgs &a, hipStream_t st) {
+    return gate_shape<SCORED ? 16 : 32>(a.n, [&](auto lpr, auto epl) {
         constexpr int L = lpr, E = epl;
         const int per_group = a.n / a.n_groups, lanes = per_group / E;
         const bool whole = L > 1 && a.n_groups > 1 && per_group % E == 0 && (lanes & (lanes - 1)) == 0 && lanes < L;     // groups of whole lanes
         const dim3 grid(gate_blocks(a.rows, 256 / L));
-        if (scored && whole) hipLaunchKernelGGL((k_gate_fwd<T, L, E, true, (L > 1)>), grid, dim3(256), 0, st, weights, cells, a);
-        else if (scored) hipLaunchKernelGGL((k_gate_fwd<T, L, E, true, false>), grid, dim3(256), 0, st, weights, cells, a);
-        else if (whole) hipLaunchKernelGGL((k_gate_fwd<T, L, E, false, (L > 1)>), grid, dim3(256), 0, st, weights, cells, a);
-        else hipLaunchKernelGGL((k_gate_fwd<T, L, E, false, false>), grid, dim3(256), 0, st, weights, cells, a);
+        if (whole) hipLaunchKernelGGL((k_gate_fwd<T, L, E, SCORED, (L > 1)>), grid, dim3(256), 0, st, weights, cells, a);
+        else hipLaunchKernelGGL((k_gate_fwd<T, L, E, SCORED, false>), grid, dim3(256), 0, st, weights, cells, a);
         return check_launch("k_gate_fwd");
     });
 }
+template <class T> static int gate_forward(float *weights, int32_t *cells, const GateArgs &a, hipStream_t st) {
+    const bool scored = a.bias || (a.n_groups > 1 && a.group_top > 1);
+    return scored ? gate_forward_as<T, true>(weights, cells, a, st) : gate_forward_as<T, false>(weights, cells, a, st);
+}
 template <class T>
 static int gate_backward(void *dx, int64_t ldd, const float *dw, int64_t lddw, const int32_t *cells, const GateArgs &a, hipStream_t st) {
-    return gate_shape(a.n, [&](auto lpr, auto epl) {
+    return gate_shape<32>(a.n, [&](auto lpr, auto epl) {
         constexpr int L = lpr, E = epl;
         hipLaunchKernelGGL((k_gate_bwd<T, L, E>), dim3(gate_blocks(a.rows, 256 / L)), dim3(256), 0, st, (T *)dx, ldd, dw, lddw, cells, a);
         return check_launch("k_gate_bwd");
