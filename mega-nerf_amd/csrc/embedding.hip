@@ -105,16 +105,16 @@ __global__ __launch_bounds__(256) void k_emb_sum(void *__restrict__ grad, int gr
     else if (cur != padding) emb_write<T>(grad, (int64_t)cur * width + c, acc, m, scale, grad_f32);
 }
 
-// The tile in which a run begins that goes on behind it owns the run: tail[t] + head[t + 1] + ... + head[the tile of its end].  A
-// workgroup looks at 16 tiles; a run of up to EMB_SHORT more tiles is joined by one wave, a longer one by the whole workgroup.  Eight
-// lanes share a sum's columns, whatever the width, and the columns are spread over workgroups: so a run over a sixth of 65521 rows
-// (676 tiles of 512 columns) is added up by 8 workgroups in 32 phases each (64 lanes and 4 phases: 77 us).
-constexpr int EMB_JOIN = 16, EMB_SHORT = 16;
+// The tile in which a run begins that goes on behind it owns the run: tail[t] + head[t + 1] + ... + head[the tile of its end].  Runs of up
+// to EMB_SHORT more tiles: a wave per tile.  Longer ones: workgroups of their own (blockIdx.y > 0) that look over 64 tiles at once and
+// add a run up with 8 lanes across and 32 phases, the columns spread over blockIdx.y: a run over a sixth of 65521 rows (676 tiles of 512
+// columns) took 77 us with one workgroup of 4 phases.
+constexpr int EMB_SHORT = 16, EMB_LOOK = 64;
 
 // head[u0], head[u0 + step] ... up to head[last], added to acc
 template <class T>
 __device__ __forceinline__ void emb_add_heads(float (&acc)[Vec<T>::N], const float *head, int64_t u0, int64_t step, int64_t last, int width, int c, int m) {
-#pragma unroll 8
+#pragma unroll 4
     for (int64_t u = u0; u <= last; u += step)
 #pragma unroll
         for (int i = 0; i < Vec<T>::N; i += 4) {
@@ -125,91 +125,94 @@ __device__ __forceinline__ void emb_add_heads(float (&acc)[Vec<T>::N], const flo
         }
 }
 
+// the key of the run that tile t owns, -1 if it owns none; `further`: whether the run goes on behind tile t + EMB_SHORT
+__device__ __forceinline__ int emb_owned(const int32_t *keys, int64_t t, int64_t n, int64_t padding, bool &further) {
+    const int64_t p0 = t * EMB_TILE, p1 = p0 + EMB_TILE, far = p1 + EMB_SHORT * EMB_TILE;
+    further = false;
+    if (p1 >= n) return -1;
+    const int k = keys[p1 - 1], next = keys[p1], first = keys[p0], before = p0 > 0 ? keys[p0 - 1] : -1, there = far < n ? keys[far] : -1;
+    if (next != k || k == padding || (first == k && before == k)) return -1;
+    further = there == k;
+    return k;
+}
+
 template <class T, int LPR>
 __global__ __launch_bounds__(256) void k_emb_join(void *__restrict__ grad, int grad_f32, const float *__restrict__ head,
                                                   const float *__restrict__ tail, const int32_t *__restrict__ keys, int64_t n, int width,
-                                                  int64_t padding, float scale) {
-    constexpr int V = Vec<T>::N, PH = 256 / LPR, WPH = 64 / LPR;
-    __shared__ float lds[PH][LPR * V];
-    __shared__ int owner[EMB_JOIN], spans[EMB_JOIN], longer[EMB_JOIN], n_long;
-    const int lane = threadIdx.x % LPR, ph = threadIdx.x / LPR, wave = threadIdx.x >> 6, wph = (threadIdx.x & 63) / LPR;
-    const int c = ((int)blockIdx.y * LPR + lane) * V, m = width - c;
+                                                  int64_t padding, float scale, int short_y) {
+    constexpr int V = Vec<T>::N;
+    __shared__ float lds[256 * V];
+    __shared__ int keys_of[EMB_LOOK];
     const int64_t tiles = (n + EMB_TILE - 1) / EMB_TILE;
-    for (int64_t b0 = (int64_t)blockIdx.x * EMB_JOIN; b0 < tiles - 1; b0 += (int64_t)gridDim.x * EMB_JOIN) {
-        __syncthreads();                               // the last round's lists have been read
-        if (threadIdx.x == 0) n_long = 0;
-        if (threadIdx.x < EMB_JOIN) {
-            // tile t owns a run if its last key goes on behind it and did not fill it from before its beginning
-            const int64_t t = b0 + threadIdx.x, p1 = (t + 1) * EMB_TILE;
-            int k = -1;
-            if (p1 < n) {
-                const int64_t p0 = t * EMB_TILE;
-                k = keys[p1 - 1];
-                if (keys[p1] != k || k == padding || (p0 > 0 && keys[p0] == k && keys[p0 - 1] == k)) k = -1;
-            }
-            owner[threadIdx.x] = k;
-        }
-        __syncthreads();
-        for (int o = wave; o < EMB_JOIN; o += 4) {
-            const int k = owner[o];
-            if (k < 0) continue;
-            // the run's last tile: the first tile from t + 1 on that the run does not leave (lane i looks at tile t + 1 + i)
-            const int64_t t = b0 + o, mark = (t + 2 + (threadIdx.x & 63)) * EMB_TILE;
-            const uint64_t leaves = __ballot(mark >= n || keys[mark < n ? mark : n - 1] != k);
-            const int more = leaves ? __ffsll((unsigned long long)leaves) : 65;          // tiles behind t, 65: more than 64
-            if (more > EMB_SHORT) {
-                if ((threadIdx.x & 63) == 0) longer[atomicAdd(&n_long, 1)] = o;
-                if ((threadIdx.x & 63) == 0) spans[o] = leaves ? more : 0;
-                continue;
-            }
+    if ((int)blockIdx.y < short_y) {
+        constexpr int WPH = 64 / LPR;
+        const int lane = threadIdx.x % LPR, ph = (threadIdx.x & 63) / LPR;
+        const int c = ((int)blockIdx.y * LPR + lane) * V, m = width - c;
+        float *mine = lds + (threadIdx.x >> 6) * 64 * V;                     // [WPH][LPR * V] of this wave
+        for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < tiles - 1; t += (int64_t)gridDim.x * 4) {
+            bool further;
+            const int k = emb_owned(keys, t, n, padding, further);
+            if (k < 0 || further) continue;                                  // (the whole wave alike)
+            // lane i: does the run leave tile t + 1 + i?  The first that it leaves is its last
+            const int64_t mark = (t + 2 + (threadIdx.x & 63)) * EMB_TILE;
+            const int more = __ffsll((unsigned long long)__ballot(mark >= n || keys[mark < n ? mark : n - 1] != k));
             float acc[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = 0.f;
-            if (wph == 0) emb_add_heads<T>(acc, tail, t, 1, t, width, c, m);
-            emb_add_heads<T>(acc, head, t + 1 + wph, WPH, t + more, width, c, m);
-            // phases of this wave in order (no other wave touches these rows of lds)
-            wave_sync();
+            if (ph == 0) emb_add_heads<T>(acc, tail, t, 1, t, width, c, m);
+            emb_add_heads<T>(acc, head, t + 1 + ph, WPH, t + more, width, c, m);
+            if constexpr (WPH > 1) {
+                wave_sync();
 #pragma unroll
-            for (int i = 0; i < V; ++i) lds[ph][lane * V + i] = acc[i];
-            wave_sync();
-            if (wph == 0 && m > 0) {
-                for (int q = 1; q < WPH; ++q)
+                for (int i = 0; i < V; ++i) mine[ph * LPR * V + lane * V + i] = acc[i];
+                wave_sync();
+                if (ph == 0)
+                    for (int q = 1; q < WPH; ++q)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) acc[i] += lds[ph + q][lane * V + i];
-                emb_write<T>(grad, (int64_t)k * width + c, acc, m, scale, grad_f32);
+                        for (int i = 0; i < V; ++i) acc[i] += mine[q * LPR * V + lane * V + i];
             }
+            if (ph == 0 && m > 0) emb_write<T>(grad, (int64_t)k * width + c, acc, m, scale, grad_f32);
         }
+        return;
+    }
+    constexpr int PH = 32;
+    const int lane = threadIdx.x % 8, ph = threadIdx.x / 8;
+    const int c = (((int)blockIdx.y - short_y) * 8 + lane) * V, m = width - c;
+    for (int64_t b0 = (int64_t)blockIdx.x * EMB_LOOK; b0 < tiles - 1; b0 += (int64_t)gridDim.x * EMB_LOOK) {
         __syncthreads();
-        for (int l = 0; l < n_long; ++l) {             // (in any order: every run is its own row)
-            const int o = longer[l], k = owner[o];
+        bool further = false;
+        int own = -1;
+        if (threadIdx.x < EMB_LOOK) own = emb_owned(keys, b0 + threadIdx.x, n, padding, further);
+        if (threadIdx.x < EMB_LOOK) keys_of[threadIdx.x] = further ? own : -1;
+        if (!__syncthreads_or(further)) continue;
+        for (int o = 0; o < EMB_LOOK; ++o) {
+            const int k = keys_of[o];
+            if (k < 0) continue;                                             // (the whole workgroup alike)
             const int64_t t = b0 + o;
-            int64_t last = t + spans[o];
-            if (spans[o] == 0) {
-                // first place behind the run, in [lo, hi]: 256 probes at a time (each place before it holds k, none behind it)
-                int64_t lo = (t + 2) * EMB_TILE, hi = n;
-                while (lo < hi) {
-                    const int64_t each = (hi - lo + 255) / 256, at = lo + each * threadIdx.x;
-                    const int64_t in = __syncthreads_count(at < hi && keys[at < hi ? at : lo] == k);         // probes inside the run
-                    if (in == 0) { hi = lo; break; }
-                    const int64_t from = lo + each * (in - 1) + 1, upto = lo + each * in;
-                    lo = from;
-                    hi = upto < hi ? upto : hi;
-                }
-                last = (hi - 1) / EMB_TILE;
+            // first place behind the run, in [lo, hi]: 256 probes at a time (each place before it holds k, none behind it)
+            int64_t lo = (t + 1 + EMB_SHORT) * EMB_TILE + 1, hi = n;
+            while (lo < hi) {
+                const int64_t each = (hi - lo + 255) / 256, at = lo + each * threadIdx.x;
+                const int64_t in = __syncthreads_count(at < hi && keys[at < hi ? at : lo] == k);         // probes inside the run
+                if (in == 0) { hi = lo; break; }
+                const int64_t upto = lo + each * in;
+                lo += each * (in - 1) + 1;
+                hi = upto < hi ? upto : hi;
             }
+            const int64_t last = (hi - 1) / EMB_TILE;
             float acc[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = 0.f;
             if (ph == 0) emb_add_heads<T>(acc, tail, t, 1, t, width, c, m);
             emb_add_heads<T>(acc, head, t + 1 + ph, PH, last, width, c, m);
-            __syncthreads();                           // the last run's sums have been read
+            __syncthreads();                                                 // the last run's sums have been read
 #pragma unroll
-            for (int i = 0; i < V; ++i) lds[ph][lane * V + i] = acc[i];
+            for (int i = 0; i < V; ++i) lds[ph * 8 * V + lane * V + i] = acc[i];
             __syncthreads();
             if (ph == 0 && m > 0) {
                 for (int q = 1; q < PH; ++q)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) acc[i] += lds[q][lane * V + i];
+                    for (int i = 0; i < V; ++i) acc[i] += lds[q * 8 * V + lane * V + i];
                 emb_write<T>(grad, (int64_t)k * width + c, acc, m, scale, grad_f32);
             }
         }
@@ -252,12 +255,13 @@ static int emb_backward(void *grad, int grad_f32, const void *dy, int64_t ldy, i
     return emb_lanes(width, Vec<T>::N, [&](auto lpr) {
         constexpr int L = lpr;
         const unsigned gy = (unsigned)((width + L * Vec<T>::N - 1) / (L * Vec<T>::N));
-        const int64_t per = 256 / L, joins = (tiles - 1 + EMB_JOIN - 1) / EMB_JOIN;
+        const int64_t per = 256 / L, joins = (tiles - 1 + 3) / 4;
         hipLaunchKernelGGL((k_emb_sum<T, L>), dim3((unsigned)((tiles + per - 1) / per), gy), dim3(256), 0, st, grad, grad_f32, head, tail, (const T *)dy,
                            ldy, keys, order, rows, width, padding, scale);
+        const unsigned gl = tiles > EMB_SHORT ? (unsigned)((width + 8 * Vec<T>::N - 1) / (8 * Vec<T>::N)) : 0;
         if (tiles > 1)
-            hipLaunchKernelGGL((k_emb_join<T, 8>), dim3((unsigned)(joins < 65536 ? joins : 65536), (unsigned)((width + 8 * Vec<T>::N - 1) / (8 * Vec<T>::N))),
-                               dim3(256), 0, st, grad, grad_f32, head, tail, keys, rows, width, padding, scale);
+            hipLaunchKernelGGL((k_emb_join<T, L>), dim3((unsigned)(joins < 1024 ? joins : 1024), gy + gl), dim3(256), 0, st, grad, grad_f32, head, tail, keys,
+                               rows, width, padding, scale, (int)gy);
         return check_launch("k_emb_sum / k_emb_join");
     });
 }

@@ -230,6 +230,23 @@ def test_embedding_long_runs(order, dtype):
     check_embedding(idx, torch.randn(count, width, generator=g).to(dtype), torch.randn(n, width, generator=g).to(dtype), 4.5)
 
 
+def test_embedding_runs_over_many_tiles():
+    """Runs of thousands of tiles (their ends are searched for), beside short ones, in narrow and wide tables."""
+    g = gen(13)
+    for n, width, share in ((200003, 5, 0.9), (70001, 140, 0.5), (30000, 600, 0.7)):
+        idx = torch.where(torch.rand(n, generator=g) < share, torch.randint(1, 4, (n,), generator=g) * 7, torch.randint(300, (n,), generator=g))
+        check_long(idx, torch.randn(n, width, generator=g), 300)
+
+
+def check_long(idx, dy, count):
+    """Sums of up to 10^5 rows: 16 in a tile, then tiles / 32 in a phase, 32 phases."""
+    from mega_nerf.embedding import embedding_backward
+    grad = embedding_backward(dy.to(DEV), idx.to(DEV), count)
+    s = torch.zeros(count, dy.shape[1], dtype=torch.float64).index_add_(0, idx, dy.double())
+    sa = torch.zeros(count, dy.shape[1], dtype=torch.float64).index_add_(0, idx, dy.double().abs())
+    within(grad, s, (16 + len(idx) / 512 + 40) * U * sa)
+
+
 def test_embedding_index_types_padding_and_clamping():
     from mega_nerf.embedding import embedding, embedding_backward, embedding_forward
     g = gen(12)
@@ -368,6 +385,22 @@ def test_gate_groups(n, groups, k_groups, k, score):
         x, bias, dw, mask = gate_inputs(13, n, k, torch.float32, n + top)
         for how in (dict(), dict(bias=bias), dict(bias=bias, mask=mask), dict(mask=mask)):
             check_gate(x, k, dw, score=score, n_groups=groups, k_groups=k_groups, group_top=top, scale=1.5, **how)
+
+
+@pytest.mark.parametrize('n,groups', [(256, 8), (300, 1), (25, 1)])
+def test_gate_more_rows_than_workgroups(n, groups):
+    from mega_nerf.gating import route_topk_backward, route_topk_forward
+    g = torch.Generator(DEV).manual_seed(n)
+    rows = 140000 if n > 32 else 2200000
+    x, bias = torch.randn(rows, n, device=DEV, generator=g).to(torch.bfloat16), 0.2 * torch.randn(n, device=DEV, generator=g)
+    how = dict(score='sigmoid', bias=bias, n_groups=groups, k_groups=max(1, groups // 2), group_top=2)
+    w, c = route_topk_forward(x, 3, **how)
+    dw = torch.randn(rows, 3, device=DEV, generator=g)
+    dx = route_topk_backward(dw, x, c, score='sigmoid')
+    for part in (slice(0, 50), slice(rows // 2, rows // 2 + 50), slice(rows - 37, rows)):
+        w2, c2 = route_topk_forward(x[part].clone(), 3, **how)
+        assert torch.equal(w[part], w2) and torch.equal(c[part], c2)
+        assert torch.equal(dx[part], route_topk_backward(dw[part].clone(), x[part].clone(), c2, score='sigmoid'))
 
 
 def test_gate_ties_go_to_the_lowest_cell():
@@ -547,6 +580,13 @@ def check_product(m, n, k, dtype, bias, relu, seed, a=None, b=None):
                                    (64, 64, 64), (65, 257, 130), (100, 128, 1040), (129, 127, 65), (200, 300, 16), (256, 256, 256), (257, 511, 513),
                                    (515, 260, 640), (1000, 256, 319), (700, 1025, 1)])
 def test_product_against_64_bits(m, n, k):
+    for i, dtype in enumerate(TYPES):
+        check_product(m, n, k, dtype, bias=i != 1, relu=i == 2, seed=m + n + k)
+
+
+@pytest.mark.parametrize('m,n,k', [(12289, 1100, 200), (12300, 1030, 64), (49200, 250, 33), (2000, 1000, 333), (1500, 1100, 1), (3000, 800, 512)])
+def test_product_many_tiles(m, n, k):
+    """Enough tiles for the 256 x 256 and the 128 x 128 kernels, whole and ragged, from one step of K to an odd number of them."""
     for i, dtype in enumerate(TYPES):
         check_product(m, n, k, dtype, bias=i != 1, relu=i == 2, seed=m + n + k)
 
