@@ -11,10 +11,6 @@ namespace mnr {
 typedef _Float16 f16_t;
 typedef __bf16 bf16_t;
 
-template <class T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
-template <class T> __device__ __forceinline__ T from_f(float v) { return (T)v; }        // to nearest, ties to even
-
-inline size_t type_size(int t) { return t == MNR_F32 ? 4 : 2; }
 inline bool type_ok(int t) { return t == MNR_F32 || t == MNR_F16 || t == MNR_BF16; }
 
 // One element of a vector of runtime type (norm weights, biases: read once per wave, so the switch costs nothing)

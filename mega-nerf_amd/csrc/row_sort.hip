@@ -4,7 +4,7 @@
 // k_sort_count counts digits per workgroup, k_sort_scan turns the counts into positions, k_sort_place ranks and writes.  Inside a
 // wave a lane's rank is the number of lower lanes with its digit, from one ballot per bit.  Counts are whole numbers, so the order
 // does not depend on which workgroup ran first.  Keys of b bits take ceil(b / 11) passes of equal width: 2048 counters a wave are 32 KB of
-// LDS, and 2000 images sort in one pass (3 launches; two passes of 8 bits took 52 us for 196608 rows).  Up to 4096 rows one workgroup
+// LDS, and 2000 images sort in one pass (3 launches: 22 us for 196608 rows, two passes of 8 bits took 52).  Up to 4096 rows one workgroup
 // does all passes in LDS (one launch).  At the sizes here the passes cost their launches and the ranking, not their bytes.
 #include "row_sort.h"
 
