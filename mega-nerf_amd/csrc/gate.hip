@@ -328,7 +328,7 @@ template <class T, int EPL> __device__ __forceinline__ void gate_exact(const Gat
 
 // LPR lanes share a row, lane t holds cells t EPL ... and slots t, t + LPR, ...
 template <class T, int LPR, int EPL, bool SCORED, bool LANES>
-__global__ __launch_bounds__(256, SCORED ? 2 : 4) void k_gate_fwd(float *__restrict__ weights, int32_t *__restrict__ cells, GateArgs a) {
+__global__ __launch_bounds__(256, SCORED ? 2 : 3) void k_gate_fwd(float *__restrict__ weights, int32_t *__restrict__ cells, GateArgs a) {
     constexpr int RPB = 256 / LPR, MAX_K = LPR * EPL < GATE_MAX_K ? LPR * EPL : GATE_MAX_K;
     __shared__ int chosen[RPB][MAX_K + 1];             // (+1: a column's entries fall into different banks)
     const int t = threadIdx.x % LPR, e0 = t * EPL;
