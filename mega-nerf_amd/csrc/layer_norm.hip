@@ -250,7 +250,8 @@ __global__ __launch_bounds__(256) void k_ln_fwd_wide(T *__restrict__ y, int64_t 
 #pragma unroll
             for (int i = 0; i < V; ++i) s += v[i];
         }
-        float mean = row_sum<256>(s, lds) / (float)C, d = 0.f;
+        const float mean = row_sum<256>(s, lds) / (float)C;
+        float d = 0.f;                                 // the mean's correction, kept apart from it to the end: their sum rounds to fp32
         for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 256 * V) {
             const int n = part(c);
             load_part<T>(v, xr + c, n);
@@ -263,9 +264,8 @@ __global__ __launch_bounds__(256) void k_ln_fwd_wide(T *__restrict__ y, int64_t 
         }
         d = row_sum<256>(d, lds) / (float)C;
         const float rstd = 1.f / sqrtf(fmaxf(row_sum<256>(q, lds) / (float)C - d * d, 0.f) + eps);
-        mean += d;
         if (threadIdx.x == 0) {
-            if (mean_out) mean_out[r] = mean;
+            if (mean_out) mean_out[r] = mean + d;
             if (rstd_out) rstd_out[r] = rstd;
         }
         for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 256 * V) {
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256) void k_ln_fwd_wide(T *__restrict__ y, int64_t 
             float wv[V], bv[V];
             ln_affine<V>(wv, bv, w, b, wtype, c, n);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = (v[i] - mean) * rstd * wv[i] + bv[i];
+            for (int i = 0; i < V; ++i) v[i] = (v[i] - mean - d) * rstd * wv[i] + bv[i];
             store_part<T>(y + r * ldy + c, v, n);
         }
     }

@@ -128,6 +128,15 @@ def test_layer_norm_far_from_zero_constant_rows_and_nan():
     assert torch.isnan(y[1]).all() and torch.isnan(y[2]).all() and torch.isfinite(y[[0, 3, 4]]).all()
 
 
+def test_wide_layer_norm_far_from_zero():
+    """Rows wider than a workgroup's registers keep their precision on a mean of 10^4 as narrow ones do: with the corrected mean rounded
+    to fp32 (half a step of 10^4 is 4.9e-4, in units of the spread of 1) y was off by 4e-4; the bound below is 4e-6 at h = 0."""
+    for rows, C in ((21, 4100), (3, 20001)):
+        g = gen(C)
+        x = torch.randn(rows, C, generator=g) + 10000.0
+        check_norm(x, None, None, torch.randn(rows, C, generator=g))
+
+
 def test_layer_norm_strided_rows_and_offsets():
     from mega_nerf.layer_norm import layer_norm_backward, layer_norm_forward
     g = gen(7)
