@@ -3,7 +3,7 @@ nerf.py:84-85,149 outside the fused kernels, in any width and type.  The sums of
 (``mnr_scatter_rows`` of the layer-by-layer path adds with atomics: its last bits change from run to run).
 
 ``embedding`` is the differentiable call; ``embedding_forward`` / ``embedding_backward`` are its passes for callers with a tape of their
-own, and may be recorded into a HIP graph."""
+own: they record nothing for autograd, and may be recorded into a HIP graph."""
 from __future__ import annotations
 
 from typing import Optional

@@ -4,7 +4,7 @@ distance to the cells' centroids; this one goes by scores that a layer has compu
 the cells and blend weights, per cell the list of its rows.
 
 ``route_topk`` is the differentiable call; ``route_topk_forward`` / ``route_topk_backward`` are its passes for callers with a tape of
-their own, and may be recorded into a HIP graph."""
+their own: they record nothing for autograd, and may be recorded into a HIP graph."""
 from __future__ import annotations
 
 from typing import Optional, Tuple

@@ -2,8 +2,8 @@
 plain ReLU layers (nerf.py:62-113) is normalised with, beside the layer-by-layer kernels of csrc/layerwise.hip.
 
 ``layer_norm`` is the differentiable call.  ``layer_norm_forward`` / ``layer_norm_backward`` are its two passes for callers that keep
-their own tape (as models.layerwise does); they may be recorded into a HIP graph, which the autograd node refuses: a graph's backward
-pass is recorded from the explicit call."""
+their own tape (as models.layerwise does): they record nothing for autograd, whatever their inputs require, and may be recorded into a
+HIP graph, which the autograd node refuses: a graph's backward pass is recorded from the explicit call."""
 from __future__ import annotations
 
 from typing import Optional, Tuple

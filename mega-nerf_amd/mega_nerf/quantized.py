@@ -1,6 +1,7 @@
 """Matrix product in 8-bit integers with a scale for every row of the input and every output channel (csrc/int8_product.hip): the dense
 layers of a wide model served at a quarter of the bytes and on the 8-bit matrix pipe, beside the fp32 products of csrc/tgemm.hip and
-csrc/layerwise.hip.  Inference only: quantisation has no gradient here."""
+csrc/layerwise.hip.  Inference only: quantisation has no gradient here.  A parameter counts as a constant; what a recorded computation
+has produced is refused, since its gradient would end here without a word."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional
@@ -21,11 +22,17 @@ class QuantizedRows(NamedTuple):
         return self.values.float() * self.scale[:, None]
 
 
+def _refuse_recorded(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.grad_fn is not None for t in tensors):
+        raise NotImplementedError('{} is inference-only (use torch.no_grad())'.format(what))
+
+
 def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     """``x`` [rows, cols] (float32, float16, bfloat16) with the scale max|row| / 127 for each row; values are rounded to the nearest,
     ties to even.  A row of zeros gets scale 0; a row that holds an inf or NaN gets scale NaN.  A weight [out, in] is quantised the
     same way, once: its rows are the output channels.  The values' rows start 128 bytes apart or a multiple of it, zeros in between
     (what the product reads fastest)."""
+    _refuse_recorded('quantize_rows', x)
     code = N.element_type(x, 'x')
     if x.dim() != 2 or x.shape[1] == 0:
         raise N.NativeError('quantize_rows expects [rows, cols] with a column at least (got {})'.format(tuple(x.shape)))
@@ -76,6 +83,7 @@ def int8_product(a: QuantizedRows, b: QuantizedRows, bias: Optional[torch.Tensor
                  out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """[M, N] = a [M, K] times the transpose of b [N, K] (+ bias float32 [N], ReLU): the integer sums are exact (K <= 131071), scaled in
     fp32 and rounded once to ``out_dtype``."""
+    _refuse_recorded('int8_product', a.scale, b.scale, bias)
     av, sa, m, k, lda = _operand(a, 'a', True)
     bv, sb, n, kb, ldb = _operand(b, 'weight', False)
     N.on_device_of(av, bv, 'weight')
@@ -95,6 +103,7 @@ def int8_linear(x: torch.Tensor, weight: QuantizedRows, bias: Optional[torch.Ten
     ``out_dtype``."""
     if x.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError('int8_linear is inference-only (use torch.no_grad())')
+    _refuse_recorded('int8_linear', weight.scale, bias)
     xcode = N.element_type(x, 'x')
     shape = x.shape
     if x.dim() == 0 or shape[-1] == 0:

@@ -44,6 +44,23 @@ def test_int8_linear_refuses_gradients():
         int8_linear(torch.zeros(2, 8, requires_grad=True), QuantizedRows(torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4)))
 
 
+def test_quantised_calls_refuse_what_a_recorded_computation_produced():
+    """Its gradient would be lost; a parameter is a constant, and nothing is recorded under no_grad (those calls get as far as the device)."""
+    leaf = torch.zeros(4, 8, requires_grad=True)
+    values, scale, bias = torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4, requires_grad=True), torch.zeros(4, requires_grad=True)
+    q, const = QuantizedRows(values, scale.detach()), torch.zeros(2, 8)
+    for call in (lambda: quantize_rows(leaf * 2), lambda: int8_linear(const, q, bias * 2), lambda: int8_linear(const, QuantizedRows(values, scale * 2)),
+                 lambda: int8_product(q, q, bias * 2), lambda: int8_product(QuantizedRows(values, scale * 2), q),
+                 lambda: int8_product(q, QuantizedRows(values, scale * 2))):
+        with pytest.raises(NotImplementedError, match='inference-only'):
+            call()
+        with torch.no_grad(), pytest.raises(N.NativeError, match='HIP device'):
+            call()
+    for call in (lambda: quantize_rows(leaf), lambda: int8_linear(const, QuantizedRows(values, scale), bias), lambda: int8_product(q, q, bias)):
+        with pytest.raises(N.NativeError, match='HIP device'):
+            call()
+
+
 def test_captured_backward_is_refused(monkeypatch):
     monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
     with pytest.raises(N.NativeError, match='route_topk_backward'):
