@@ -14,6 +14,7 @@ import torch
 from mega_nerf import _native as N
 
 _SCORES = {'softmax': 0, 'sigmoid': 1}
+_MAX_K, _MAX_DISPATCH = 32, (1 << 24) - 1
 
 
 def _score(score: str) -> int:
@@ -27,6 +28,19 @@ def _logits(logits: torch.Tensor):
     if logits.dim() < 1 or logits.shape[-1] == 0:
         raise N.NativeError('logits must be [..., cells] with a cell at least (got {})'.format(tuple(logits.shape)))
     return (code,) + tuple(N.matrix(logits))
+
+
+def _choice(logits: torch.Tensor, k: int, n_groups: int, k_groups: int, group_top: int) -> None:
+    """Before anything is allocated, and before ctypes takes numbers of 2^32 and more for their low 32 bits."""
+    n = logits.shape[-1]
+    if not 1 <= k <= min(n, _MAX_K):
+        raise N.NativeError('route_topk chooses 1 to {} cells, at most as many as there are (got {} of {})'.format(_MAX_K, k, n))
+    if not 1 <= n_groups <= n or n % n_groups:
+        raise N.NativeError('n_groups must divide the cells evenly (got {} for {} cells)'.format(n_groups, n))
+    if not 1 <= k_groups <= n_groups or k > k_groups * (n // n_groups):
+        raise N.NativeError('k_groups must be 1 to n_groups and its groups hold k cells (got {} of {} groups, k {})'.format(k_groups, n_groups, k))
+    if group_top not in (1, 2):
+        raise N.NativeError('group_top must be 1 or 2 (got {})'.format(group_top))
 
 
 def _mask(mask: Optional[torch.Tensor], logits: torch.Tensor):
@@ -55,9 +69,11 @@ def route_topk_forward(logits: torch.Tensor, k: int, score: str = 'softmax', bia
     lie in groups of neighbours, and only the ``k_groups`` groups stay open whose ``group_top`` (1 or 2) best s + bias sum highest.
     weights = scale * s, over the sum of the chosen s if ``renormalise``.
 
-    Fewer than k open cells: the slots left over hold cell -1 with weight 0.  A NaN among a row's open logits (softmax: or +inf) gives
-    that row cells -1 and weights NaN."""
+    k is 1 to 32, of up to 1024 cells.  Fewer than k open cells: the slots left over hold cell -1 with weight 0.  A NaN among a row's
+    open logits (softmax: or +inf) gives that row cells -1 and weights NaN."""
     sc = _score(score)
+    if logits.dim() and logits.shape[-1]:
+        _choice(logits, k, n_groups, k_groups, group_top)
     code, x, rows, n, ldl = _logits(logits)
     m, ldm = _mask(mask, logits)
     if bias is not None:
@@ -125,11 +141,13 @@ def dispatch(cells: torch.Tensor, n_cells: int) -> Tuple[torch.Tensor, torch.Ten
     host synchronisation."""
     if cells.dtype != torch.int32:
         raise N.NativeError('cells must be int32 (got {})'.format(cells.dtype))
+    if not 1 <= n_cells <= _MAX_DISPATCH:
+        raise N.NativeError('dispatch needs 1 to {} cells (got {})'.format(_MAX_DISPATCH, n_cells))
     N.require_device(cells, 'cells')
     cells = cells.contiguous()
     slots = cells.numel()
     order = cells.new_empty(slots)
-    offsets = cells.new_empty(max(int(n_cells), 0) + 1)
+    offsets = cells.new_empty(int(n_cells) + 1)
     lib = N.lib()
     size = lib.mnr_gate_dispatch_workspace_bytes(slots, n_cells)
     ws = cells.new_empty(size, dtype=torch.uint8)

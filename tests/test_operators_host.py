@@ -61,6 +61,23 @@ def test_quantised_calls_refuse_what_a_recorded_computation_produced():
             call()
 
 
+def test_counts_are_checked_before_anything_is_allocated():
+    """... and as whole numbers: a C int takes the low 32 bits of a larger one, so 2^32 + 2 cells a row were two."""
+    x, c = torch.zeros(3, 8), torch.zeros(3, 2, dtype=torch.int32)
+    for how, text in ((dict(k=0), 'chooses'), (dict(k=-1), 'chooses'), (dict(k=9), 'chooses'), (dict(k=2 ** 32 + 2), 'chooses'),
+                      (dict(k=1, n_groups=0), 'n_groups'), (dict(k=1, n_groups=3), 'n_groups'), (dict(k=1, n_groups=2 ** 32 + 1), 'n_groups'),
+                      (dict(k=1, n_groups=4, k_groups=5), 'k_groups'), (dict(k=1, n_groups=4, k_groups=2 ** 32 + 1), 'k_groups'),
+                      (dict(k=3, n_groups=4, k_groups=1), 'hold k'), (dict(k=1, group_top=3), 'group_top'), (dict(k=1, group_top=2 ** 32 + 1), 'group_top')):
+        for call in (route_topk, route_topk_forward):
+            with pytest.raises(N.NativeError, match=text):
+                call(x, **how)
+    with pytest.raises(N.NativeError, match='chooses'):
+        route_topk_forward(torch.zeros(2, 64), 33)
+    for n in (0, -1, 1 << 24, 2 ** 32 + 5):
+        with pytest.raises(N.NativeError, match='dispatch needs'):
+            dispatch(c, n)
+
+
 def test_captured_backward_is_refused(monkeypatch):
     monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
     with pytest.raises(N.NativeError, match='route_topk_backward'):
