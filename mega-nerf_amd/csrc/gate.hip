@@ -535,6 +535,7 @@ __global__ void k_gate_no_offsets(int32_t *__restrict__ offsets, int n) {
 // lanes and cells per lane for n cells: the fewest lanes at up to MOST (32, or 16 where scores are compared: with 32 those kernels take
 // 220 registers, two waves a SIMD) values each
 template <int MOST, class F> static int gate_shape(int n, F &&f) {
+    static_assert(MOST == 16 || MOST == 32, "64 lanes of 16 cells or 32 lanes of 32 hold the most there are");
     using std::integral_constant;
     if (n <= 8) return f(integral_constant<int, 1>{}, integral_constant<int, 8>{});
     if (n <= 16) return f(integral_constant<int, 1>{}, integral_constant<int, 16>{});
@@ -543,8 +544,11 @@ template <int MOST, class F> static int gate_shape(int n, F &&f) {
     if (n <= 4 * MOST) return f(integral_constant<int, 4>{}, integral_constant<int, MOST>{});
     if (n <= 8 * MOST) return f(integral_constant<int, 8>{}, integral_constant<int, MOST>{});
     if (n <= 16 * MOST) return f(integral_constant<int, 16>{}, integral_constant<int, MOST>{});
-    if (n <= 32 * MOST) return f(integral_constant<int, 32>{}, integral_constant<int, MOST>{});
-    return f(integral_constant<int, 64>{}, integral_constant<int, 1024 / 64>{});
+    if constexpr (MOST == 32) return f(integral_constant<int, 32>{}, integral_constant<int, MOST>{});       // (1024 cells, the most there are)
+    else {
+        if (n <= 32 * MOST) return f(integral_constant<int, 32>{}, integral_constant<int, MOST>{});
+        return f(integral_constant<int, 64>{}, integral_constant<int, MOST>{});
+    }
 }
 
 static unsigned gate_blocks(int64_t rows, int rpb) {

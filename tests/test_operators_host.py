@@ -224,6 +224,35 @@ def test_every_argument_list_matches_the_header():
         assert list(getattr(lib, name).argtypes) == want, name
 
 
+def test_gate_kernels_are_the_ones_that_calls_reach():
+    """A lane holds 8, 16 or 32 cells where the logits decide and in the gradient, 8 or 16 where scores do; up to that many cells are one
+    lane's, beyond it lanes double up to 1024 cells.  No other shape is built."""
+    import importlib.util
+    import re
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    spec = importlib.util.spec_from_file_location('kernel_resources', root / 'mega-nerf_amd' / 'tools' / 'kernel_resources.py')
+    kr = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(kr)
+    if not kr.tools_available():
+        pytest.skip('llvm-objdump not found')
+
+    def shape(n, most):
+        per = next(e for e in (8, 16, most) if n <= e or e == most)
+        lanes = 1
+        while lanes * per < n:
+            lanes *= 2
+        return lanes, per
+
+    shapes = {most: {shape(n, most) for n in range(1, 1025)} for most in (16, 32)}
+    built = {'k_gate_bwd': set(), False: set(), True: set()}
+    for k in kr.kernel_resources(N.LIB_PATH):
+        m = re.match(r'_ZN3mnr10(k_gate_[a-z]+)I(f|DF16_|DF16b|u6__bf16)Li(\d+)ELi(\d+)E(?:Lb([01])ELb[01]E)?E', k['symbol'])
+        if m:
+            built['k_gate_bwd' if m[1] == 'k_gate_bwd' else m[5] == '1'].add((int(m[3]), int(m[4])))
+    assert built == {'k_gate_bwd': shapes[32], False: shapes[32], True: shapes[16]}
+
+
 def test_no_kernel_holds_packed_fp32_arithmetic():
     """v_pk_add / mul / fma_f32 have given wrong values on these GPUs: no code object of the library holds one (the build forbids them;
     tgemm.hip, built without that flag, must be free of them by itself)."""
