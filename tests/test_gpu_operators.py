@@ -600,6 +600,15 @@ def test_product_many_tiles(m, n, k):
         check_product(m, n, k, dtype, bias=i != 1, relu=i == 2, seed=m + n + k)
 
 
+@pytest.mark.parametrize('m,n,k', [(4352, 4096, 64), (4400, 4300, 100), (4352, 4097, 1), (8300, 4700, 333),
+                                   (38400, 250, 333), (24000, 500, 64), (38000, 256, 1)])
+def test_product_more_tiles_than_workgroups(m, n, k):
+    """Workgroups that take a second and a third tile: 272, 306, 289 and 627 tiles of 256 x 256 on 256 workgroups, 600, 752 and 594 tiles
+    of 128 x 128 on 512, whole and ragged, K of one step, with a tail and of an uneven number of steps."""
+    for i, dtype in enumerate(TYPES):
+        check_product(m, n, k, dtype, bias=i != 1, relu=i == 2, seed=m + n + k)
+
+
 def test_product_extremes_and_long_sums():
     full = lambda r, c, v: torch.full((r, c), v, dtype=torch.int8)      # noqa: E731
     check_product(3, 70, 131071, torch.float32, False, False, 1, full(3, 131071, -128), full(70, 131071, -128))     # 2^31 - 2^14: the largest sum
