@@ -104,6 +104,17 @@ def test_layer_norm_against_64_bits(rows, C, dtype):
     check_norm(x, 1 + 0.2 * torch.randn(C, generator=g), 0.1 * torch.randn(C, generator=g), dy)
 
 
+@pytest.mark.parametrize('rows,C,dtype', [(130, 4100, torch.float32), (4099, 4100, torch.float32), (2500, 8192, torch.float32), (2100, 8200, torch.bfloat16),
+                                          (2500, 2052, torch.float32), (6000, 1100, torch.float32), (2100, 4100, torch.bfloat16), (4700, 2056, torch.float16)])
+def test_layer_norm_many_wide_rows(rows, C, dtype):
+    """Rows that a workgroup shares (1025 to 4096 columns of fp32, 2049 to 8192 of 16 bits) or reads over and over (wider ones), in more
+    rows than workgroups: several turns of the row loops, several strips of rows whose column sums are joined, a ragged last strip."""
+    g = gen(rows + C)
+    x = (torch.randn(rows, C, generator=g) * 1.7 + 0.4).to(dtype)
+    dy = torch.randn(rows, C, generator=g).to(dtype)
+    check_norm(x, 1 + 0.2 * torch.randn(C, generator=g), 0.1 * torch.randn(C, generator=g), dy)
+
+
 @pytest.mark.parametrize('wdtype', TYPES + [None])
 def test_layer_norm_weight_types_and_none(wdtype):
     g = gen(5)
