@@ -407,6 +407,16 @@ def test_gate_groups(n, groups, k_groups, k, score):
             check_gate(x, k, dw, score=score, n_groups=groups, k_groups=k_groups, group_top=top, scale=1.5, **how)
 
 
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('n,groups,k_groups,k', [(1024, 2, 1, 8), (512, 2, 1, 8), (512, 4, 3, 8), (32, 2, 1, 3)])
+def test_gate_groups_of_many_lanes(n, groups, k_groups, k, score):
+    """Groups of 1, 8, 16 and 32 whole lanes."""
+    for top in (1, 2):
+        x, bias, dw, mask = gate_inputs(13, n, k, torch.float32, n + top)
+        for how in (dict(), dict(bias=bias), dict(bias=bias, mask=mask), dict(mask=mask)):
+            check_gate(x, k, dw, score=score, n_groups=groups, k_groups=k_groups, group_top=top, scale=1.5, **how)
+
+
 @pytest.mark.parametrize('n,groups', [(256, 8), (300, 1), (25, 1)])
 def test_gate_more_rows_than_workgroups(n, groups):
     from mega_nerf.gating import route_topk_backward, route_topk_forward
