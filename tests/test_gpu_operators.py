@@ -417,6 +417,19 @@ def test_gate_groups_of_many_lanes(n, groups, k_groups, k, score):
             check_gate(x, k, dw, score=score, n_groups=groups, k_groups=k_groups, group_top=top, scale=1.5, **how)
 
 
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('n,groups,k_groups,k', [(256, 8, 4, 8), (256, 1, 1, 8), (8, 1, 1, 2), (25, 5, 2, 3)])
+def test_gate_with_a_bias_of_zeros(n, groups, k_groups, k, score):
+    """A balance bias as training starts with it: scores tie wherever 16-bit logits do, in every row where all logits are alike."""
+    g = gen(n + groups)
+    fine = (1.5 * torch.randn(150, n, generator=g)).to(torch.bfloat16)
+    coarse = torch.randn(150, n, generator=g).mul(4).round().div(4)
+    for x in (fine, coarse.to(torch.bfloat16), coarse.to(torch.float16), torch.zeros(70, n), torch.full((70, n), -2.5).to(torch.bfloat16)):
+        for top in (1, 2):
+            for bias in (torch.zeros(n), torch.full((n,), 0.25)):
+                check_gate(x, k, torch.randn(len(x), k, generator=g), score=score, bias=bias, n_groups=groups, k_groups=k_groups, group_top=top)
+
+
 @pytest.mark.parametrize('n,groups', [(256, 8), (300, 1), (25, 1)])
 def test_gate_more_rows_than_workgroups(n, groups):
     from mega_nerf.gating import route_topk_backward, route_topk_forward
