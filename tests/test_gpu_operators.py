@@ -545,6 +545,21 @@ def test_dispatch_is_the_stable_order(slots, n_cells):
     assert torch.equal(offsets.cpu().long(), torch.searchsorted(key.sort().values, torch.arange(n_cells + 1)))
 
 
+@pytest.mark.parametrize('slots', [1100003, 2100001])
+def test_orders_of_more_rows_than_two_to_the_20(slots):
+    """2048 and 4096 rows a workgroup of the sort, in one pass and in two, under the dispatch and under the table's gradient."""
+    from mega_nerf.gating import dispatch
+    g = gen(slots)
+    for n_cells in (25, 70000):
+        cells = torch.randint(-1, n_cells, (slots,), generator=g, dtype=torch.int32)
+        order, offsets = dispatch(cells.to(DEV), n_cells)
+        key = torch.where(cells < 0, n_cells, cells.long())
+        ordered, want = torch.sort(key, stable=True)
+        assert torch.equal(order.cpu().long(), want)
+        assert torch.equal(offsets.cpu().long(), torch.searchsorted(ordered, torch.arange(n_cells + 1)))
+        check_embedding(torch.randint(n_cells, (slots,), generator=g), torch.randn(n_cells, 3, generator=g), torch.randn(slots, 3, generator=g), 0.5)
+
+
 def test_dispatch_one_cell_and_none():
     from mega_nerf.gating import dispatch
     for fill in (-1, 0, 3, 6):
