@@ -806,6 +806,41 @@ def passes():
             ('product', lambda: (int8_linear(x, wq),)), ('product one row', lambda: (int8_linear(x[:1], wq),))]
 
 
+def test_one_dimensional_inputs_and_expanded_gradients():
+    """One row without a row dimension, and the gradient of a sum: one value for all elements, no pitch at all."""
+    from mega_nerf.embedding import embedding, embedding_forward
+    from mega_nerf.gating import dispatch, route_topk, route_topk_forward
+    from mega_nerf.layer_norm import layer_norm, layer_norm_forward
+    from mega_nerf.quantized import int8_linear, quantize_rows
+    g = gen(40)
+    x, table = torch.randn(5, 40, generator=g).to(DEV), torch.randn(9, 40, generator=g).to(DEV)
+    wq = quantize_rows(torch.randn(24, 40, generator=g).to(DEV))
+    col = x.t().contiguous().t()[2]                          # a row whose elements lie five apart
+    for row in (x[2], col):
+        assert torch.equal(layer_norm_forward(row)[0], layer_norm_forward(x)[0][2])
+        w, c = route_topk_forward(row, 3)
+        w2, c2 = route_topk_forward(x, 3)
+        assert torch.equal(w, w2[2]) and torch.equal(c, c2[2])
+        assert torch.equal(int8_linear(row, wq), int8_linear(x, wq)[2])
+    assert torch.equal(dispatch(c, 40)[0].cpu().long(), torch.sort(c.cpu(), stable=True).indices)
+    assert torch.equal(embedding_forward(torch.tensor(4, device=DEV), table, 2.0), table[4] * 2)
+    for shape in ((5, 40), (40,), (2, 3, 40)):
+        leaves = [torch.randn(shape, generator=gen(41)).to(DEV).requires_grad_() for _ in range(2)]
+        for leaf, full in zip(leaves, (False, True)):
+            y = torch.cat([layer_norm(leaf), route_topk(leaf, 32, renormalise=False)[0]], -1)
+            if full:
+                y.backward(torch.ones_like(y))
+            else:
+                y.sum().backward()
+        assert torch.equal(leaves[0].grad, leaves[1].grad)
+    t1, t2 = table.clone().requires_grad_(), table.clone().requires_grad_()
+    idx = torch.randint(9, (4, 6), generator=g).to(DEV)
+    embedding(idx, t1).sum().backward()
+    y = embedding(idx, t2)
+    y.backward(torch.ones_like(y))
+    assert torch.equal(t1.grad, t2.grad) and float((t1.grad.sum(1).cpu() - 40 * torch.bincount(idx.cpu().view(-1), minlength=9)).abs().max()) == 0
+
+
 def test_every_pass_in_a_graph_replayed():
     todo = passes()
     eager = [[t.clone() for t in f()] for _, f in todo]
