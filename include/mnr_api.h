@@ -217,8 +217,8 @@ int mnr_layer_norm_backward(void *dx_dev, int64_t lddx, void *dw_dev, void *db_d
  * Indices outside the table are clamped, as in mnr_gather_rows. */
 int mnr_embedding_forward(void *out_dev, int64_t ldo, const void *table_dev, int64_t ldt, int64_t count, int64_t width, const void *idx_dev,
                           int idx_type, float scale, int64_t rows, int type, void *stream);
-/* grad [count][width], dense and overwritten: grad[v] = scale sum of dy[r] over the rows r with idx[r] = v, in row order (the rows are
- * sorted by index: mnr_scatter_rows adds them up with atomics instead).  The row of padding_idx (-1: none) stays zero.
+/* grad [count][width], dense and overwritten: grad[v] = scale sum of dy[r] over the rows r with idx[r] = v, in a fixed order (the rows
+ * are sorted by index: mnr_scatter_rows adds them up with atomics instead).  The row of padding_idx (-1: none) stays zero.
  * grad_type: type, or MNR_F32. */
 size_t mnr_embedding_backward_workspace_bytes(int64_t rows, int64_t count, int64_t width);
 int mnr_embedding_backward(void *grad_dev, int grad_type, const void *dy_dev, int64_t ldy, const void *idx_dev, int idx_type, int64_t rows,

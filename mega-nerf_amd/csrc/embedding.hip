@@ -2,11 +2,13 @@
 //
 //   out[r] = scale table[idx[r]]             grad[v] = scale sum_{r : idx[r] = v} dy[r]
 //
-// Bound by HBM.  The lookup reads 16 bytes per lane wherever the row starts.  The gradient sorts the rows by index (row_sort.hip,
-// stable; the sort's first launch clears the gradient) and walks the sorted order in tiles of 16 rows: a lane group keeps its columns' fp32 sum of the run it is in, and writes it once when
-// the index changes.  A run that crosses tiles leaves one fp32 sum per tile, joined by k_emb_join in tile order.  No atomics: sums
-// are in row order, the same bits every time, and a popular index costs what an unpopular one does.  196608 rows of 48 fp32 columns in
-// runs of 192: lookup 11.5 us, sort 22, sums 8, joins 15; 65521 rows of 512 bf16 columns, skewed: 19, 35, 17 and 24 us.
+// The lookup is bound by HBM: 16 bytes per lane wherever the row starts.  The gradient sorts the rows by index (row_sort.hip, stable; the
+// sort's first launch clears the gradient) and walks the sorted order in tiles of 16 rows: a lane group keeps its columns' fp32 sum of
+// the run it is in, and writes it once when the index changes.  A run that crosses tiles leaves one fp32 sum per tile, joined by
+// k_emb_join.  No atomics: inside a tile rows are added in row order, tiles in interleaved phases that width, type and the run's length
+// fix, so the same inputs give the same bits.  What bounds the gradient is the sort and the joins, not its bytes: 196608 rows of 48 fp32
+// columns in runs of 192 take 11.5 us for the lookup, 22 to sort, 8 for the sums and 15 for the joins; 65521 rows of 512 bf16 columns,
+// skewed so that long runs hold most of them, 19, 35, 17 and 24 us.
 #include "row_sort.h"
 
 namespace mnr {

@@ -1,6 +1,6 @@
 """Table lookup with a scale, and the table's gradient by sorted indices (csrc/embedding.hip): the per-image appearance vectors of
-nerf.py:84-85,149 outside the fused kernels, in any width and type.  The sums of a popular index are in row order and free of atomics
-(``mnr_scatter_rows`` of the layer-by-layer path adds with atomics: its last bits change from run to run).
+nerf.py:84-85,149 outside the fused kernels, in any width and type.  Sums are free of atomics and in a fixed order: the same inputs give
+the same bits (``mnr_scatter_rows`` of the layer-by-layer path adds with atomics: its last bits change from run to run).
 
 ``embedding`` is the differentiable call; ``embedding_forward`` / ``embedding_backward`` are its passes for callers with a tape of their
 own: they record nothing for autograd, and may be recorded into a HIP graph."""
