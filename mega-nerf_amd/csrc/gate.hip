@@ -7,13 +7,17 @@
 //   gradient (cells fixed), g = scale dw:    softmax, renormalised: dx_j = p_j (g_j - sum p g) over the chosen, p = w / scale
 //       softmax: dx_e = s_e (g_e [e chosen] - sum_chosen s g);   sigmoid: dx_j = s_j (1 - s_j) g_j, renormalised p_j (1 - s_j) (g_j - sum p g)
 //
-// Bound by HBM for few cells (a row is read once), by the instructions of the arg-max rounds for many.  A lane holds up to 32 neighbouring
-// cells in registers, so up to 32 cells need no exchange at all (a thread is a row) and 256 cells 8 lanes: a round is a local maximum, a
-// DPP maximum over the lanes and a ballot that names the lowest lane that has it.  (With 4 cells a lane and 8 lanes a row every
-// instruction served 8 rows instead of 64: 25 cells took 20 us; 8 cells and 32 lanes: 256 cells 122 us.)  Where no score enters a comparison the values are the logits themselves (exact).  Otherwise the
-// scores are formed in fp32 and every decision is checked: a row where two values that a decision kept apart are closer than fp32's
-// error is decided again in 64 bits, by the whole wave, so the choice is always the one of the definition (all rows in 64 bits: 256
-// cells in 8 groups, 65536 rows of bf16 took 266 us; so it is 93).  25 cells, 196608 rows: 16 us forward, 16.5 us backward.
+// Bound by HBM for few cells (a row is read once), by the instructions of the arg-max rounds for many.  A lane holds neighbouring cells in
+// registers, up to 32 where the logits decide and in the gradient (a thread is a row of up to 32 cells, 256 cells are 8 lanes), up to 16
+// where scores do (256 cells are 16 lanes): a round is a local maximum, a DPP maximum over the lanes and a ballot that names the lowest
+// lane that has it.  (With 4 cells a lane and 8 lanes a row every instruction served 8 rows instead of 64: 25 cells took 20 us; 8 cells
+// and 32 lanes: 256 cells 122 us.)  25 cells, 196608 rows: 16 us forward, 16.5 us backward.
+// Where no score enters a comparison the values are the logits themselves (exact).  Otherwise the scores are formed in fp32 and every
+// decision is checked: a row where two values that a decision kept apart are closer than fp32's error is decided again in 64 bits, so the
+// choice is the one of the definition (all rows in 64 bits: 65536 rows of 256 bf16 cells in 8 groups took 266 us; checked, 86 to 93).
+// Such rows go one after the other through their wave, and equal scores are among them although the lowest index already decides there:
+// the same 65536 rows take 243 us with a bias of zeros (16-bit logits tie in about a third of them) and 395 us where all logits are equal too,
+// 196608 rows of 8 fp32 cells 9.4, 9.6 and 115 us, of 25 bf16 cells 20.6, 26.6 and 121 us.
 // Weights are formed from the logits of the chosen (log-sigmoids for sigmoid), so renormalising never divides by an underflowed sum.
 #include <type_traits>
 
