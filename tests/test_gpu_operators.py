@@ -841,6 +841,109 @@ def test_one_dimensional_inputs_and_expanded_gradients():
     assert torch.equal(t1.grad, t2.grad) and float((t1.grad.sum(1).cpu() - 40 * torch.bincount(idx.cpu().view(-1), minlength=9)).abs().max()) == 0
 
 
+class Guarded:
+    """A buffer [rows, pitch] inside a larger one, filled with a byte pattern: what a call may write is ``cols`` of each row."""
+
+    def __init__(self, rows, cols, pitch, dtype, lead=1):
+        self.rows, self.cols, self.pitch = rows, cols, pitch
+        self.raw = torch.full(((rows + 2) * pitch + lead,), 0, dtype=dtype, device=DEV)
+        self.raw.view(torch.uint8).fill_(0xa5)
+        self.body = self.raw[pitch + lead:pitch + lead + rows * pitch].view(rows, pitch)
+        self.before = self.raw.clone()
+
+    def ptr(self):
+        return self.body.data_ptr()
+
+    def result(self):
+        """The rows, after a check that nothing else has changed."""
+        out = self.body[:, :self.cols].clone()
+        self.body[:, :self.cols] = self.before[:1]
+        assert torch.equal(self.raw.view(torch.uint8), self.before.view(torch.uint8))
+        self.body[:, :self.cols] = out
+        return out
+
+
+def same_bits(a, b):
+    return a.shape == b.shape and torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_entries_write_their_rows_and_their_workspace_alone(dtype):
+    """The C entries with pitches wider than their rows, rows that start at any element and workspaces of exactly the bytes they ask for:
+    the results of the tight calls, and not a byte changed behind a row, before the first, behind the last or behind the workspace."""
+    from mega_nerf import _native as N
+    from mega_nerf import embedding as E, gating as G, layer_norm as L, quantized as Q
+    lib, code, g = N.lib(), N.ELEMENT_TYPES[dtype], gen(50)
+
+    def call(fn, *args):
+        N.launch(torch.empty(0, device=DEV), fn, *args)
+
+    def space(size):
+        return Guarded(1, size, size + 256, torch.uint8, lead=(-(size + 256)) % 256)
+
+    for rows, C in ((1, 7), (21, 63), (70, 64), (333, 129), (1000, 319), (5, 4100), (3, 8200)):
+        x, dy = (torch.randn(rows, C, generator=g).to(DEV, dtype) for _ in range(2))
+        w, b = torch.randn(C, generator=g).to(DEV), torch.randn(C, generator=g).to(DEV)
+        y, m, r = L.layer_norm_forward(x, w, b)
+        out = Guarded(rows, C, C + 5, dtype)
+        call(lib.mnr_layer_norm_forward, out.ptr(), C + 5, None, None, x.data_ptr(), C, w.data_ptr(), b.data_ptr(), rows, C, 1e-5, code, 0)
+        assert same_bits(out.result(), y)
+        size = lib.mnr_layer_norm_backward_workspace_bytes(rows, C, code)
+        dx, ws = Guarded(rows, C, C + 3, dtype), space(size)
+        dw, db = Guarded(1, C, C, torch.float32), Guarded(1, C, C, torch.float32)
+        call(lib.mnr_layer_norm_backward, dx.ptr(), C + 3, dw.ptr(), db.ptr(), dy.data_ptr(), C, x.data_ptr(), C, w.data_ptr(), m.data_ptr(), r.data_ptr(), rows, C,
+             code, 0, ws.ptr(), size)
+        ws.result()
+        for a, c in zip((dx, dw, db), L.layer_norm_backward(dy, x, w, m, r)):
+            assert same_bits(a.result().view(c.shape), c)
+    for rows, count, width in ((1, 1, 1), (50, 7, 33), (4096, 90, 17), (5000, 3, 40), (9000, 5001, 20), (70000, 257, 5)):
+        idx = torch.randint(count, (rows,), generator=g).to(DEV)
+        table, dy = torch.randn(count, width, generator=g).to(DEV, dtype), torch.randn(rows, width, generator=g).to(DEV, dtype)
+        out = Guarded(rows, width, width + 3, dtype)
+        call(lib.mnr_embedding_forward, out.ptr(), width + 3, table.data_ptr(), width, count, width, idx.data_ptr(), 4, 2.0, rows, code)
+        assert same_bits(out.result(), E.embedding_forward(idx, table, 2.0))
+        size = lib.mnr_embedding_backward_workspace_bytes(rows, count, width)
+        ws, grad = space(size), Guarded(1, count * width, count * width + (count * width) % 2, dtype, lead=0)
+        call(lib.mnr_embedding_backward, grad.ptr(), code, dy.data_ptr(), width, idx.data_ptr(), 4, rows, count, width, -1, 2.0, code, ws.ptr(), size)
+        ws.result()
+        assert same_bits(grad.result().view(count, width), E.embedding_backward(dy, idx, count, 2.0))
+    for rows, n, k in ((1, 8, 2), (70, 25, 3), (33, 100, 8), (9, 300, 5), (3, 1000, 32)):
+        x, bias, dwt = torch.randn(rows, n, generator=g).to(DEV, dtype), torch.randn(n, generator=g).to(DEV), torch.randn(rows, k, generator=g).to(DEV)
+        for b in (None, bias):
+            wt, ce = Guarded(1, rows * k, rows * k, torch.float32), Guarded(1, rows * k, rows * k, torch.int32)
+            call(lib.mnr_gate_forward, wt.ptr(), ce.ptr(), x.data_ptr(), n, N.ptr(b), None, 0, rows, n, k, 0, 1, 1, 1, 0, 1.5, code)
+            w2, c2 = G.route_topk_forward(x, k, bias=b, renormalise=False, scale=1.5)
+            assert same_bits(wt.result().view(rows, k), w2) and same_bits(ce.result().view(rows, k), c2)
+        dx = Guarded(rows, n, n + 7, dtype)
+        call(lib.mnr_gate_backward, dx.ptr(), n + 7, dwt.data_ptr(), k, x.data_ptr(), n, c2.data_ptr(), None, 0, rows, n, k, 0, 0, 1.5, code)
+        assert same_bits(dx.result(), G.route_topk_backward(dwt, x, c2, renormalise=False, scale=1.5))
+    for slots, n in ((1, 1), (4096, 300), (4097, 25), (70001, 5000)):
+        cells = torch.randint(-1, n, (slots,), generator=g, dtype=torch.int32).to(DEV)
+        size = lib.mnr_gate_dispatch_workspace_bytes(slots, n)
+        ws, order, offsets = space(size), Guarded(1, slots, slots, torch.int32), Guarded(1, n + 1, n + 1, torch.int32)
+        call(lib.mnr_gate_dispatch, order.ptr(), offsets.ptr(), cells.data_ptr(), slots, n, ws.ptr(), size)
+        ws.result()
+        for a, c in zip((order, offsets), G.dispatch(cells, n)):
+            assert same_bits(a.result().view(-1), c)
+    for m, n, k in ((1, 33, 100), (40, 70, 319), (300, 129, 64), (2000, 1001, 80), (4200, 3300, 48)):
+        x, w = torch.randn(m, k, generator=g).to(DEV, dtype), Q.quantize_rows(torch.randn(n, k, generator=g).to(DEV))
+        pitch = (k + 15) // 16 * 16
+        values, scale = Guarded(m, pitch, pitch, torch.int8, lead=(-pitch) % 256), Guarded(1, m, m, torch.float32)
+        call(lib.mnr_quantize_rows, values.ptr(), pitch, scale.ptr(), x.data_ptr(), k, m, k, code)
+        q = Q.quantize_rows(x)
+        held = values.result()
+        assert same_bits(held[:, :k], q.values) and float(held[:, k:].abs().sum()) == 0 and same_bits(scale.result().view(-1), q.scale)
+        size, ldb = lib.mnr_int8_linear_workspace_bytes(m, k), w.values.stride(0)
+        y, ws = Guarded(m, n, n + 5, dtype), space(size)
+        call(lib.mnr_int8_linear, y.ptr(), n + 5, x.data_ptr(), k, code, w.values.data_ptr(), ldb, w.scale.data_ptr(), None, m, n, k, 1, code, ws.ptr(), size)
+        ws.result()
+        want = Q.int8_linear(x, w, relu=True)
+        assert same_bits(y.result(), want)
+        y = Guarded(m, n, n + 2, dtype)
+        call(lib.mnr_int8_product, y.ptr(), n + 2, held.data_ptr(), pitch, q.scale.data_ptr(), w.values.data_ptr(), ldb, w.scale.data_ptr(), None, m, n, k, 1, code)
+        assert same_bits(y.result(), want)
+
+
 def test_every_pass_in_a_graph_replayed():
     todo = passes()
     eager = [[t.clone() for t in f()] for _, f in todo]
