@@ -83,7 +83,7 @@ def int8_product(a: QuantizedRows, b: QuantizedRows, bias: Optional[torch.Tensor
                  out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """[M, N] = a [M, K] times the transpose of b [N, K] (+ bias float32 [N], ReLU): the integer sums are exact (K <= 131071), scaled in
     fp32 and rounded once to ``out_dtype``."""
-    _refuse_recorded('int8_product', a.scale, b.scale, bias)
+    _refuse_recorded('int8_product', a[1], b[1], bias)
     av, sa, m, k, lda = _operand(a, 'a', True)
     bv, sb, n, kb, ldb = _operand(b, 'weight', False)
     N.on_device_of(av, bv, 'weight')
@@ -103,7 +103,7 @@ def int8_linear(x: torch.Tensor, weight: QuantizedRows, bias: Optional[torch.Ten
     ``out_dtype``."""
     if x.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError('int8_linear is inference-only (use torch.no_grad())')
-    _refuse_recorded('int8_linear', weight.scale, bias)
+    _refuse_recorded('int8_linear', weight[1], bias)
     xcode = N.element_type(x, 'x')
     shape = x.shape
     if x.dim() == 0 or shape[-1] == 0:

@@ -61,6 +61,14 @@ def test_quantised_calls_refuse_what_a_recorded_computation_produced():
             call()
 
 
+def test_a_plain_pair_is_a_quantised_operand():
+    """(values, scale) without the name, as before: such calls get as far as the device."""
+    pair = (torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4))
+    for call in (lambda: int8_linear(torch.zeros(2, 8), pair), lambda: int8_product(pair, pair)):
+        with pytest.raises(N.NativeError, match='HIP device'):
+            call()
+
+
 def test_counts_are_checked_before_anything_is_allocated():
     """... and as whole numbers: a C int takes the low 32 bits of a larger one, so 2^32 + 2 cells a row were two."""
     x, c = torch.zeros(3, 8), torch.zeros(3, 2, dtype=torch.int32)
